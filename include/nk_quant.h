@@ -1,0 +1,112 @@
+/*
+ * nk_quant.h — the quantised decode step of libnkgemm.so (sm_100a): linears with 4-bit weights,
+ * and a KV cache held in 8 bits with the append that fills it and the attention that reads it.
+ * They stand beside nk_gemm_bf16 (nk_gemm.h), nk_qk_norm_rope_cache_bf16 and
+ * nk_attention_decode_bf16 (nk_decode.h), move a quarter and half of their bytes, and share
+ * their conventions: device pointers, a cudaStream_t, 0 or NK_ERR_* returned before anything is
+ * launched, no allocation, no host synchronisation, capture-safe, programmatic dependent launch.
+ * The reference engine is bf16 throughout and has no counterpart of these.
+ */
+#ifndef NK_QUANT_H
+#define NK_QUANT_H
+
+#include "nk_gemm.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* ---- 4-bit weights with group scales ------------------------------------------------------
+ *
+ *   y[m, n] = bf16_rne( sum_k x[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group] )
+ *
+ * q: 4-bit codes 0..15, s: bf16 or fp16 scales, z: zero points 0..15 (8 when there are none);
+ * differences and products exact, sums in fp32, one rounding at the end.
+ *
+ * Storage, laid out once when the weights are loaded (KB = ceil(K / 128), NB = ceil(N / 16),
+ * GP = KB * 128 / group; codes, scales and zero points past K or N are 0):
+ *   codes:  [NB][KB][2][32] 16-byte pieces. Piece (i, b, half, lane) holds row
+ *           n = 16 i + 8 half + lane / 4; its 32-bit word j (0..3) holds
+ *           k = 128 b + 32 j + 8 (lane % 4) + 0..7: element 2 p in bits [4p, 4p + 4) and element
+ *           2 p + 1 in bits [16 + 4p, 20 + 4p), p = 0..3. One warp load of a piece row is 512
+ *           contiguous bytes, and masking (word >> 4p) with 0x000f000f gives one operand
+ *           register of the matrix instruction.
+ *   scales: [NB][GP][8][2] 16-bit, element (i, g, r, half) of row 16 i + 8 half + r.
+ *   zeros:  [NB][GP][8][2] bytes, same order (NULL: every zero point is 8).
+ */
+#define NK_W4_SCALE_BF16 0
+#define NK_W4_SCALE_FP16 1
+
+/* Bytes of the three arrays above (0 for arguments out of range: N, K >= 1, group 32, 64 or
+ * 128). */
+NK_API size_t nk_w4_code_bytes(int N, int K);
+NK_API size_t nk_w4_scale_bytes(int N, int K, int group);
+NK_API size_t nk_w4_zero_bytes(int N, int K, int group);
+
+/* x: [M, K] bf16, row stride ldx >= K (elements); y: [M, N] bf16, row stride ldy >= N. codes and
+ * scales 16-byte aligned, zeros 2-byte aligned or NULL; x and y 2-byte aligned (x 16-byte aligned with
+ * ldx % 8 == 0 is read in 16-byte pieces). Any M >= 1. No workspace. The weights must have been
+ * written before the launch that precedes this one on the stream (they are read ahead of it);
+ * weights made at load time always are. */
+NK_API int nk_gemm_w4(const void* x, int64_t ldx, const void* codes, const void* scales,
+                      const void* zeros, void* y, int64_t ldy, int M, int N, int K, int group,
+                      int scale_type, nk_stream_t stream);
+
+/* ---- KV cache in 8 bits -------------------------------------------------------------------
+ *
+ * Keys and values are e4m3 codes (1 byte, finite range +-448) times a scale held for each
+ * (sequence, kv head, block of `block` token slots), in fp32 [batch][kv_heads][ceil(capacity /
+ * block)]. block is 16, 32, 64 or 128. Code arrays have unit stride along the 128 head
+ * elements and any batch, head and token strides that are multiples of 16 (bytes).
+ * capacity <= 2^30.
+ *
+ * `position` is a device int64 array: entry b (or entry 0 for every sequence when
+ * per_sequence == 0) is the slot of sequence b's first new token; `tokens` (1..16) new tokens take
+ * slots position .. position + tokens - 1. A negative position marks an idle sequence.
+ * A position with position + tokens > capacity is treated as idle and sets the device error
+ * word to NK_ERR_RANGE (nk_device_error).
+ */
+#define NK_Q8_MAX_TOKENS 16
+#define NK_Q8_MAX_BATCH 1024
+
+/* Per-head RMSNorm and RoPE of the new tokens' query and key heads exactly as
+ * nk_qk_norm_rope_cache_bf16 rounds them; queries to q_out, keys and values appended to the
+ * cache. For each block that the new tokens touch, with amax their largest finite magnitude
+ * in it: scale = max(former scale if the block holds earlier tokens, smallest power of two
+ * s >= 2^-64 with amax <= 448 s, 0 for amax = 0). When the scale rises, the earlier tokens' codes c
+ * become e4m3_rne(c * former / new); new codes are e4m3_rne(value / scale), NaN for a value
+ * that is not finite. Slots past the new tokens, and everything of an idle sequence (its q_out rows included), are
+ * left as they are.
+ *   qkv: [batch * tokens, (q_heads + 2 kv_heads) * 128] bf16, row stride ld_qkv, row b * tokens + t
+ *   q_out: [batch * tokens, q_heads * 128] bf16; q_norm, k_norm: [128]; cos, sin: [capacity, 128]
+ * bf16 pointers 8-byte aligned and ld_qkv a multiple of 4. */
+NK_API int nk_qk_norm_rope_cache_q8(const void* qkv, int64_t ld_qkv, const void* q_norm,
+                                    const void* k_norm, const void* cos_table,
+                                    const void* sin_table, const int64_t* position,
+                                    int per_sequence, void* q_out, void* k_codes, void* v_codes,
+                                    float* k_scale, float* v_scale, int batch, int tokens,
+                                    int q_heads, int kv_heads, int head_dim, int capacity,
+                                    int block, int64_t cache_batch_stride,
+                                    int64_t cache_head_stride, int64_t cache_seq_stride,
+                                    float eps, nk_stream_t stream);
+
+/* Workspace bytes of nk_attention_decode_q8, whatever the batch and capacity (0: out of range).
+ * It needs no initialisation; calls that share one must be ordered. */
+NK_API size_t nk_attention_q8_ws_bytes(int tokens, int q_heads, int kv_heads);
+
+/* Grouped attention of the new tokens over the cache: query row (b, t, h) sees slots
+ * 0 .. position + t of kv head h / (q_heads / kv_heads); fp32 scores, softmax and sums, rounded
+ * once to bf16; rows of idle sequences are zero. q, out: [batch * tokens, q_heads * 128] bf16,
+ * 8-byte aligned. q_heads / kv_heads between 1 and 16; batch <= 1024. */
+NK_API int nk_attention_decode_q8(const void* q, const void* k_codes, const void* v_codes,
+                                  const float* k_scale, const float* v_scale,
+                                  const int64_t* position, int per_sequence, void* out, int batch,
+                                  int tokens, int q_heads, int kv_heads, int head_dim,
+                                  int capacity, int block, int64_t cache_batch_stride,
+                                  int64_t cache_head_stride, int64_t cache_seq_stride,
+                                  float scale, void* ws, size_t ws_bytes, nk_stream_t stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* NK_QUANT_H */

@@ -12,7 +12,8 @@ from .gemm import (  # noqa: E402
     KIND_AUTO, KIND_GEMV, KIND_TC, KIND_GENERIC, Plan, device_error, linear_out, m_bucket, mm,
     mm_argmax, mm_f32, plan_for, workspace,
 )
+from .w4 import W4Weight, mm_w4  # noqa: E402
 
-__all__ = ["mm", "mm_argmax", "mm_f32", "linear_out", "Plan", "plan_for", "workspace",
+__all__ = ["mm", "mm_argmax", "mm_f32", "mm_w4", "W4Weight", "linear_out", "Plan", "plan_for", "workspace",
            "device_error", "m_bucket", "KIND_AUTO", "KIND_GEMV", "KIND_TC", "KIND_GENERIC"]
 __version__ = "0.1.0"

@@ -34,14 +34,16 @@ KIND_GENERIC = 3
 MAX_SPLIT = 16
 PLAN_MAGIC = 0x4E4B4731
 
-# Every function the header declares; the CPU test checks the .so exports each of them.
+# Every function the headers declare; the CPU test checks the .so exports each of them.
 EXPORTS = ("nk_plan_make", "nk_ws_bytes", "nk_ws_init", "nk_gemm_bf16", "nk_device_error",
            "nk_status_string", "nk_version", "nk_gemm_bf16_static", "nk_gemm_bf16_f32out",
            "nk_rmsnorm_bf16", "nk_qk_norm_rope_cache_bf16", "nk_attention_ws_bytes",
            "nk_attention_decode_bf16", "nk_silu_mul_bf16", "nk_peer_buffer_bytes", "nk_peer_alloc",
            "nk_peer_free", "nk_ipc_handle", "nk_ipc_open", "nk_ipc_close", "nk_allreduce_bf16",
            "nk_gemm_argmax_ws_bytes", "nk_gemm_bf16_argmax", "nk_test_withhold_partial",
-           "nk_gemm_bf16_allreduce", "nk_gemm_bf16_qkv_rope_cache")
+           "nk_gemm_bf16_allreduce", "nk_gemm_bf16_qkv_rope_cache",
+           "nk_w4_code_bytes", "nk_w4_scale_bytes", "nk_w4_zero_bytes", "nk_gemm_w4",
+           "nk_qk_norm_rope_cache_q8", "nk_attention_q8_ws_bytes", "nk_attention_decode_q8")
 
 
 NK_PEER_MAX_RANKS = 8
@@ -159,6 +161,23 @@ def load() -> ctypes.CDLL:
                                          ctypes.POINTER(NkPlan), vp, ctypes.c_size_t,
                                          ctypes.POINTER(NkPeerGroup), vp]
     L.nk_gemm_bf16_allreduce.restype = i32
+    L.nk_w4_code_bytes.argtypes = [i32, i32]
+    L.nk_w4_code_bytes.restype = ctypes.c_size_t
+    L.nk_w4_scale_bytes.argtypes = [i32, i32, i32]
+    L.nk_w4_scale_bytes.restype = ctypes.c_size_t
+    L.nk_w4_zero_bytes.argtypes = [i32, i32, i32]
+    L.nk_w4_zero_bytes.restype = ctypes.c_size_t
+    L.nk_gemm_w4.argtypes = [vp, i64, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, vp]
+    L.nk_gemm_w4.restype = i32
+    L.nk_qk_norm_rope_cache_q8.argtypes = [vp, i64, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp,
+                                           i32, i32, i32, i32, i32, i32, i32, i64, i64, i64, f32,
+                                           vp]
+    L.nk_qk_norm_rope_cache_q8.restype = i32
+    L.nk_attention_q8_ws_bytes.argtypes = [i32, i32, i32]
+    L.nk_attention_q8_ws_bytes.restype = ctypes.c_size_t
+    L.nk_attention_decode_q8.argtypes = [vp, vp, vp, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32,
+                                         i32, i32, i64, i64, i64, f32, vp, ctypes.c_size_t, vp]
+    L.nk_attention_decode_q8.restype = i32
     L.nk_device_error.argtypes = [vp, ctypes.POINTER(i32)]
     L.nk_device_error.restype = i32
     L.nk_status_string.argtypes = [i32]

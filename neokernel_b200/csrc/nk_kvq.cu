@@ -1,0 +1,811 @@
+// KV cache in 8 bits (include/nk_quant.h): the append that fills it and the attention that reads
+// it. Codes are e4m3, with one power-of-two scale per (sequence, kv head, block of tokens).
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "nk_common.cuh"
+#include "../../include/nk_quant.h"
+
+namespace nk {
+
+constexpr int kQ8MinScaleExp = -64;
+constexpr int kQ8MaxCapacity = 1 << 30;  // slot arithmetic on the host stays within 32 bits
+
+// First new slot of sequence b, or -1 where nothing is to be done for it (idle, or out of range).
+__device__ __forceinline__ int64_t q8_position(const int64_t* position, int per_sequence, int b,
+                                               int tokens, int capacity) {
+    const int64_t p = position[per_sequence ? b : 0];
+    return p < 0 || p > (int64_t)capacity - tokens ? -1 : p;
+}
+
+// ---------------------------------------------------------------------------------------
+// Append. RMSNorm + RoPE as qk_norm_rope_cache_kernel rounds them, a warp per 128-element head
+// row (lane l owns elements 4l .. 4l + 3; its RoPE partner is lane l ^ 16).
+//
+// A CTA of eight warps takes either eight query rows, or one (sequence, kv head, touched block):
+// it holds the block's new rows in registers (at most 16 tokens, two a warp), finds their
+// largest magnitudes, fixes the block's two scales, rounds earlier tokens' codes anew where a
+// scale rose, and stores. Each block belongs to one CTA, so nothing is shared between CTAs. A
+// few hundred KB move at most; the launch and two dependent round trips to memory bound it.
+// ---------------------------------------------------------------------------------------
+struct Q8AppendArgs {
+    const __nv_bfloat16* qkv; int64_t ld;
+    const __nv_bfloat16 *qn, *kn, *cos_t, *sin_t;
+    const int64_t* position; int per_sequence;
+    __nv_bfloat16* q_out;
+    uint8_t *k, *v;
+    float *ks, *vs;
+    int batch, tokens, hq, hkv, capacity, block, blocks;
+    int64_t cb, ch, cs;
+    float eps;
+    int q_ctas;                  // CTAs of query rows per sequence
+};
+
+struct Row4 { float v[4]; };
+
+__device__ __forceinline__ Row4 load_row4(const __nv_bfloat16* p) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    return Row4{{bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y)}};
+}
+
+// bf16 cast points of the decode step: the normalised value, its product with the gain, each
+// RoPE product, and their sum. The result's values are bf16 values.
+__device__ __forceinline__ Row4 q8_norm_rope(Row4 x, const __nv_bfloat16* gain,
+                                             const __nv_bfloat16* cos_r,
+                                             const __nv_bfloat16* sin_r, int lane, float eps) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss = fmaf(x.v[i], x.v[i], ss);
+    const float inv = rsqrtf(warp_sum(ss) / (float)kHeadDim + eps);
+    const Row4 w = load_row4(gain + 4 * lane), c = load_row4(cos_r + 4 * lane),
+               s = load_row4(sin_r + 4 * lane);
+    Row4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float n = bf16r(bf16r(x.v[i] * inv) * w.v[i]);
+        const float o = __shfl_xor_sync(0xffffffffu, n, 16);
+        const float rot = lane < 16 ? -o : o;
+        y.v[i] = bf16r(bf16r(n * c.v[i]) + bf16r(rot * s.v[i]));
+    }
+    return y;
+}
+
+// Smallest power of two s >= 2^-64 with amax <= 448 s (0 for 0). 448 = 1.75 * 2^8.
+__device__ __forceinline__ float q8_scale(float amax) {
+    if (amax == 0.f) return 0.f;
+    const uint32_t u = __float_as_uint(amax);
+    int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    e = max(e, kQ8MinScaleExp);
+    return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+__device__ __forceinline__ uint32_t q8_code(float v, float inv) {  // v * inv, e4m3, NaN if not finite
+    if (!(fabsf(v) <= 3.4028235e38f)) return 0x7fu;
+    return (uint32_t)__nv_cvt_float_to_fp8(v * inv, __NV_SATFINITE, __NV_E4M3);
+}
+
+__device__ __forceinline__ uint32_t q8_codes(const Row4& r, float inv) {
+    return q8_code(r.v[0], inv) | q8_code(r.v[1], inv) << 8 | q8_code(r.v[2], inv) << 16 |
+           q8_code(r.v[3], inv) << 24;
+}
+
+__device__ __forceinline__ float2 q8_decode2(uint32_t codes16) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)codes16));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+__device__ __forceinline__ uint32_t q8_requant(uint32_t codes, float ratio) {
+    const float2 a = q8_decode2(codes & 0xffffu), b = q8_decode2(codes >> 16);
+    const Row4 r{{a.x, a.y, b.x, b.y}};
+    return q8_codes(r, ratio);
+}
+
+__device__ __forceinline__ float finite_max(const Row4& r, float m) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float x = fabsf(r.v[i]);
+        if (x <= 3.4028235e38f) m = fmaxf(m, x);
+    }
+    return m;
+}
+
+constexpr int kQ8Warps = 8;
+
+__global__ void __launch_bounds__(32 * kQ8Warps) q8_append_kernel(const Q8AppendArgs a) {
+    __shared__ float s_max[2][kQ8Warps];
+    if (threadIdx.x == 0) griddep_launch_dependents();
+    griddep_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.y;
+    const int64_t raw = a.position[a.per_sequence ? b : 0];
+    const int64_t pos = q8_position(a.position, a.per_sequence, b, a.tokens, a.capacity);
+    if (pos < 0) {
+        if (raw >= 0 && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(&g_error, NK_ERR_RANGE);
+        return;
+    }
+    const int T = a.tokens;
+    if ((int)blockIdx.x < a.q_ctas) {  // query rows
+        const int row = blockIdx.x * kQ8Warps + warp;
+        if (row >= T * a.hq) return;
+        const int t = row / a.hq, h = row - t * a.hq;
+        const Row4 x = load_row4(a.qkv + ((int64_t)b * T + t) * a.ld + h * kHeadDim + 4 * lane);
+        const Row4 y = q8_norm_rope(x, a.qn, a.cos_t + (pos + t) * kHeadDim,
+                                    a.sin_t + (pos + t) * kHeadDim, lane, a.eps);
+        uint2 o;
+        o.x = pack_bf16x2(y.v[0], y.v[1]);
+        o.y = pack_bf16x2(y.v[2], y.v[3]);
+        *reinterpret_cast<uint2*>(a.q_out + (((int64_t)b * T + t) * a.hq + h) * kHeadDim + 4 * lane) = o;
+        return;
+    }
+    const int u = blockIdx.x - a.q_ctas;
+    const int h = u % a.hkv;
+    const int64_t blk = pos / a.block + u / a.hkv;
+    const int64_t s0 = blk * a.block;                            // the block's first slot
+    const int64_t lo = pos > s0 ? pos : s0;                      // its new slots [lo, hi)
+    const int64_t hi = min(pos + T, s0 + a.block);
+    if (lo >= hi) return;
+    const int n = (int)(hi - lo);
+    const bool earlier = lo > s0;
+    const int64_t si = ((int64_t)b * a.hkv + h) * a.blocks + blk;
+    const float k_old = earlier ? a.ks[si] : 0.f, v_old = earlier ? a.vs[si] : 0.f;
+    Row4 kr[2], vr[2];
+    float km = 0.f, vm = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int j = warp + i * kQ8Warps;
+        if (j < n) {
+            const int64_t slot = lo + j;
+            const __nv_bfloat16* src = a.qkv + ((int64_t)b * T + (slot - pos)) * a.ld + 4 * lane;
+            kr[i] = q8_norm_rope(load_row4(src + (int64_t)(a.hq + h) * kHeadDim), a.kn,
+                                 a.cos_t + slot * kHeadDim, a.sin_t + slot * kHeadDim, lane, a.eps);
+            vr[i] = load_row4(src + (int64_t)(a.hq + a.hkv + h) * kHeadDim);
+            km = finite_max(kr[i], km);
+            vm = finite_max(vr[i], vm);
+        }
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, off));
+        vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, off));
+    }
+    if (lane == 0) {
+        s_max[0][warp] = km;
+        s_max[1][warp] = vm;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kQ8Warps; ++w) {
+        km = fmaxf(km, s_max[0][w]);
+        vm = fmaxf(vm, s_max[1][w]);
+    }
+    const float k_new = fmaxf(k_old, q8_scale(km)), v_new = fmaxf(v_old, q8_scale(vm));
+    // scales are powers of two in [2^-64, 2^120], or 0 (every value 0): the reciprocals are exact
+    const float k_inv = k_new > 0.f ? 1.f / k_new : 0.f, v_inv = v_new > 0.f ? 1.f / v_new : 0.f;
+    const int64_t base = (int64_t)b * a.cb + (int64_t)h * a.ch + 4 * lane;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int j = warp + i * kQ8Warps;
+        if (j < n) {
+            const int64_t at = base + (lo + j) * a.cs;
+            *reinterpret_cast<uint32_t*>(a.k + at) = q8_codes(kr[i], k_inv);
+            *reinterpret_cast<uint32_t*>(a.v + at) = q8_codes(vr[i], v_inv);
+        }
+    }
+    if (threadIdx.x == 0) {
+        a.ks[si] = k_new;
+        a.vs[si] = v_new;
+    }
+    const bool k_rose = earlier && k_new != k_old, v_rose = earlier && v_new != v_old;
+    if (k_rose || v_rose) {
+        const float kq = k_old * k_inv, vq = v_old * v_inv;
+        for (int64_t slot = s0 + warp; slot < lo; slot += kQ8Warps) {
+            const int64_t at = base + slot * a.cs;
+            if (k_rose) {
+                uint32_t* p = reinterpret_cast<uint32_t*>(a.k + at);
+                *p = q8_requant(*p, kq);
+            }
+            if (v_rose) {
+                uint32_t* p = reinterpret_cast<uint32_t*>(a.v + at);
+                *p = q8_requant(*p, vq);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Attention of T new tokens over the 8-bit cache.
+//
+// Bound by the cache's bytes over HBM (a token of one kv head is 256 bytes), so every byte is read
+// once and must be requested early: the work is the list of 64-slot units of all (sequence, kv
+// head) pairs, and CTA c of the launch takes the contiguous units [U c / G, U (c + 1) / G), so
+// ragged batches leave every CTA the same number of bytes. Each of a CTA's four warps streams its
+// own 16 slots of every unit through a private ring of asynchronous copies, with no barrier
+// between warps until a pair ends.
+//
+// Per 16 slots (lane = 4 g + t): S^T = K Q^T by mma.m16n8k16 in f16 with the slots as rows and
+// up to 8 query rows (token, head of the group) per column tile. e4m3 values are exact in f16;
+// a query row is made exact there by a power of two that the score multiplies back. Softmax in fp32 with
+// running maxima. O^T += V^T P^T: V^T comes from transposed 8x8 loads of byte pairs, P^T from
+// transposing the probabilities' registers (movmatrix).
+//
+// The value scale differs between blocks, so it cannot be taken out of the sum: probabilities
+// are 2^(x + log2 s_v - my) with a running maximum my of x + log2 s_v of their own, rounded
+// to f16 (11 bits, from 2^15 down to 2^-24: what underflows is below 2^-39 of the largest
+// term), while the sum l = sum 2^(x - m) stays in fp32. Then out = (O / l) 2^(my - m).
+//
+// A pair covered by one CTA is written directly; otherwise its CTAs write (m, my, l, O) of their
+// part, and a second launch adds the parts in order of their slots.
+// ---------------------------------------------------------------------------------------
+constexpr int kQ8Unit = 64;                 // slots per unit, 16 per warp
+constexpr int kQ8AttnThreads = 128;
+constexpr int kQ8Stages = 4;                // units in flight per warp
+constexpr int kQ8WarpStage = 2 * 16 * 128;  // K and V rows of 16 slots
+constexpr int kQ8AttnSmem = kQ8Stages * 4 * kQ8WarpStage;  // 64 KB
+constexpr int kQ8MaxGrid = 148 * 4;
+constexpr int kQ8PartFloats = kHeadDim + 4; // O, m, my, l, unused
+constexpr float kQ8Shift = 15.f;            // probabilities are held times 2^15
+
+struct Q8AttnArgs {
+    const __nv_bfloat16* q;
+    const uint8_t *k, *v;
+    const float *ks, *vs;
+    const int64_t* position; int per_sequence;
+    __nv_bfloat16* out;
+    float* part;                 // [grid][2][rows][kQ8PartFloats]
+    int batch, tokens, hq, hkv, G, capacity, block, blocks;
+    int rows, row_blocks;        // query rows of a CTA (8 NT), row blocks of T * G rows
+    int grid;                    // CTAs of the first launch
+    int64_t cb, ch, cs;
+    float scale_log2;            // softmax scale times log2(e)
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t movm_t(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t v16) {  // low half of v16
+    uint32_t h;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}"
+        : "=r"(h) : "r"(v16));
+    return h;
+}
+__device__ __forceinline__ uint32_t e4m3x2_f16x2_hi(uint32_t v32) {
+    uint32_t h;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}"
+        : "=r"(h) : "r"(v32));
+    return h;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) { return exp2f(x); }
+// Factor of a part with running maximum m where all parts have maximum M. A part that saw nothing
+// (m = -inf) has sums of 0, or NaN if what it saw was NaN: 1 keeps both.
+__device__ __forceinline__ float q8_weight(float m, float M) {
+    return m == -INFINITY ? 1.f : ex2(m - M);
+}
+
+// Units of the launch, from the device positions: s_end[b] = units of sequences 0 .. b, of one
+// (kv head, row block). Every thread of the CTA calls it.
+__device__ __forceinline__ void q8_units(const Q8AttnArgs& a, int* s_end) {
+    for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
+        const int64_t p = q8_position(a.position, a.per_sequence, b, a.tokens, a.capacity);
+        s_end[b] = p < 0 ? 0 : (int)((p + a.tokens + kQ8Unit - 1) / kQ8Unit);
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {  // running sum, 32 sequences at a time
+        int base = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += 32) {
+            const int b = b0 + threadIdx.x;
+            int x = b < a.batch ? s_end[b] : 0;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, off);
+                if ((int)threadIdx.x >= off) x += y;
+            }
+            x += base;
+            if (b < a.batch) s_end[b] = x;
+            base = __shfl_sync(0xffffffffu, x, 31);
+        }
+    }
+    __syncthreads();
+}
+
+// The partition of U units over G CTAs (begin(c) = floor(U c / G)) and its inverse.
+__device__ __forceinline__ int64_t q8_begin(int64_t U, int G, int c) { return U * c / G; }
+__device__ __forceinline__ int q8_cta_of(int64_t U, int G, int64_t u) {
+    return (int)(((u + 1) * G + U - 1) / U - 1);
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kQ8AttnThreads, NT <= 2 ? 3 : 2)
+q8_attn_kernel(const Q8AttnArgs a) {
+    extern __shared__ __align__(1024) uint8_t q8_smem[];
+    __shared__ int s_end[NK_Q8_MAX_BATCH];
+    __shared__ float s_stat[4][8 * NT][4];
+    if (threadIdx.x == 0) griddep_launch_dependents();
+    griddep_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    q8_units(a, s_end);
+    const int per_b = a.hkv * a.row_blocks;                 // pairs per sequence
+    const int64_t U = (int64_t)s_end[a.batch - 1] * per_b;
+    if (blockIdx.x == 0) {
+        for (int b = threadIdx.x; b < a.batch; b += blockDim.x)
+            if (a.position[a.per_sequence ? b : 0] > (int64_t)a.capacity - a.tokens)
+                atomicExch(&g_error, NK_ERR_RANGE);
+    }
+    const int G = (int)min((int64_t)a.grid, U);             // no CTA of the partition is empty
+    if ((int)blockIdx.x >= G) return;
+    int64_t u = q8_begin(U, G, blockIdx.x);
+    const int64_t u_end = q8_begin(U, G, blockIdx.x + 1);
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(q8_smem)) +
+                          warp * (kQ8Stages * kQ8WarpStage);
+
+    while (u < u_end) {
+        // the pair of unit u: sequence b, kv head h, row block rb; its units [p0, p0 + n)
+        int lo = 0, hi = a.batch - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if ((int64_t)s_end[mid] * per_b > u) hi = mid; else lo = mid + 1;
+        }
+        const int b = lo;
+        const int64_t before = b > 0 ? (int64_t)s_end[b - 1] * per_b : 0;
+        const int n = s_end[b] - (b > 0 ? s_end[b - 1] : 0);
+        const int pr = (int)((u - before) / n);
+        const int64_t p0 = before + (int64_t)pr * n;
+        const int h = pr / a.row_blocks, rb = pr - h * a.row_blocks;
+        const int c0 = (int)(u - p0), c1 = (int)(min(u_end, p0 + n) - p0);
+        const int64_t pos = q8_position(a.position, a.per_sequence, b, a.tokens, a.capacity);
+        const int64_t len = pos + a.tokens;
+
+        const uint8_t* kb = a.k + (int64_t)b * a.cb + (int64_t)h * a.ch;
+        const uint8_t* vb = a.v + (int64_t)b * a.cb + (int64_t)h * a.ch;
+        const float* ksb = a.ks + ((int64_t)b * a.hkv + h) * a.blocks;
+        const float* vsb = a.vs + ((int64_t)b * a.hkv + h) * a.blocks;
+
+        // 16 slots of a unit: eight 16-byte pieces a row, piece c at c ^ (row & 7)
+        auto issue = [&](int c) {
+            if (c < c1) {
+                const uint32_t dst = ring + (c % kQ8Stages) * kQ8WarpStage;
+                const int64_t j0 = (int64_t)c * kQ8Unit + warp * 16;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int idx = i * 32 + lane, row = idx >> 3, piece = idx & 7;
+                    const bool ok = j0 + row < len;
+                    const int64_t off = ok ? (j0 + row) * a.cs + piece * 16 : 0;
+                    const uint32_t d = dst + row * 128 + ((piece ^ (row & 7)) * 16);
+                    cp_async<16>(d, kb + off, ok);
+                    cp_async<16>(d + 16 * 128, vb + off, ok);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < kQ8Stages - 1; ++i) issue(c0 + i);
+
+        // Q^T operand: column g of tile nt is query row 8 nt + g; dims 16 s + 4 t .. + 3 of step s
+        uint32_t qf[NT][8][2];
+        float qs[NT][2];     // 2^-shift of rows 8 nt + 2t, + 1, times the softmax scale
+        int last[NT][2];     // last slot those rows see, relative to pos (-1: no such row)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = rb * a.rows + 8 * nt + g;
+            const bool ok = r < a.tokens * a.G;
+            const int tok = ok ? r / a.G : 0, hh = ok ? r - tok * a.G : 0;
+            const __nv_bfloat16* src =
+                a.q + (((int64_t)b * a.tokens + tok) * a.hq + (int64_t)h * a.G + hh) * kHeadDim;
+            float x[8][4], m = 0.f;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                uint2 w = make_uint2(0u, 0u);
+                if (ok) w = *reinterpret_cast<const uint2*>(src + 16 * s + 4 * t);
+                x[s][0] = bf16lo(w.x); x[s][1] = bf16hi(w.x);
+                x[s][2] = bf16lo(w.y); x[s][3] = bf16hi(w.y);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(x[s][i]));
+            }
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            // largest magnitude to [2^12, 2^13): a bf16 value keeps its 8 bits down to 2^-29 of it
+            int e = (int)(__float_as_uint(m) >> 23) - 127 - 12;
+            e = min(max(e, -100), 100);
+            const float up = __uint_as_float((uint32_t)(127 - e) << 23);
+            const float down = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                qf[nt][s][0] = pack_f16x2(x[s][0] * up, x[s][1] * up);
+                qf[nt][s][1] = pack_f16x2(x[s][2] * up, x[s][3] * up);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                qs[nt][i] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + i)) * a.scale_log2;
+                const int rr = rb * a.rows + 8 * nt + 2 * t + i;
+                last[nt][i] = rr < a.tokens * a.G ? rr / a.G : -1;
+            }
+        }
+
+        float m[NT][2], my[NT][2], l[NT][2], o[8][NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = my[nt][0] = my[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
+        }
+
+        // ldmatrix rows: matrix mi = lane / 8 = (slots half mi & 1, piece + (mi >> 1)), row lane % 8
+        const int mrow = (lane >> 3 & 1) * 8 + (lane & 7), mpiece = lane >> 4;
+        for (int c = c0; c < c1; ++c) {
+            issue(c + kQ8Stages - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kQ8Stages - 1) : "memory");
+            __syncwarp();
+            const uint32_t st = ring + (c % kQ8Stages) * kQ8WarpStage;
+            const int64_t j0 = (int64_t)c * kQ8Unit + warp * 16;
+            if (j0 < len) {
+                const int blk = (int)(j0 / a.block);
+                const float k_scale = ksb[blk];
+                const float v_log2 = log2f(vsb[blk]);
+                float s[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+                for (int p = 0; p < 8; p += 2) {
+                    uint32_t r[4];
+                    ldsm_x4(st + mrow * 128 + (((p + mpiece) ^ (mrow & 7)) * 16), r);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t a0 = e4m3x2_f16x2(r[2 * i]), a2 = e4m3x2_f16x2_hi(r[2 * i]);
+                        const uint32_t a1 = e4m3x2_f16x2(r[2 * i + 1]),
+                                       a3 = e4m3x2_f16x2_hi(r[2 * i + 1]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma_f16(s[nt], a0, a1, a2, a3, qf[nt][p + i][0], qf[nt][p + i][1]);
+                    }
+                }
+                // scores of slots j0 + g, j0 + 8 + g against rows 2t, 2t + 1 of each tile
+                const int rel = (int)(j0 - pos);  // slots are seen up to pos + last
+                uint32_t pf[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[i] = s[nt][i] * (qs[nt][i & 1] * k_scale);
+                        if (rel + g + (i >> 1) * 8 > last[nt][i & 1]) x[i] = -INFINITY;
+                    }
+                    float f[2][2], al[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float mx = fmaxf(x[i], x[i + 2]);
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        const float mn = fmaxf(m[nt][i], mx);
+                        const float ref = mn == -INFINITY ? 0.f : mn;
+                        l[nt][i] = l[nt][i] * ex2(m[nt][i] - ref) + ex2(x[i] - ref) +
+                                   ex2(x[i + 2] - ref);
+                        m[nt][i] = mn;
+                        const float yn = fmaxf(my[nt][i], mx + v_log2);
+                        const float yref = yn == -INFINITY ? 0.f : yn;
+                        al[i] = ex2(my[nt][i] - yref);
+                        my[nt][i] = yn;
+                        f[0][i] = ex2(x[i] + (v_log2 - yref + kQ8Shift));
+                        f[1][i] = ex2(x[i + 2] + (v_log2 - yref + kQ8Shift));
+                    }
+                    pf[nt][0] = movm_t(pack_f16x2(f[0][0], f[0][1]));
+                    pf[nt][1] = movm_t(pack_f16x2(f[1][0], f[1][1]));
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) {
+                        o[d][nt][0] *= al[0];
+                        o[d][nt][1] *= al[1];
+                        o[d][nt][2] *= al[0];
+                        o[d][nt][3] *= al[1];
+                    }
+                }
+                // V^T: rows of tile d are dims 16 d + 2 g (first eight) and 16 d + 2 g + 1
+#pragma unroll
+                for (int p = 0; p < 8; p += 2) {
+                    uint32_t r[4];
+                    ldsm_x4_t(st + 16 * 128 + mrow * 128 + (((p + mpiece) ^ (mrow & 7)) * 16), r);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t v0 = __byte_perm(r[2 * i], 0u, 0x3120);
+                        const uint32_t v1 = __byte_perm(r[2 * i + 1], 0u, 0x3120);
+                        const uint32_t a0 = e4m3x2_f16x2(v0), a1 = e4m3x2_f16x2_hi(v0);
+                        const uint32_t a2 = e4m3x2_f16x2(v1), a3 = e4m3x2_f16x2_hi(v1);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma_f16(o[p + i][nt], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
+                    }
+                }
+            }
+            __syncwarp();  // the stage may be refilled
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+        // sums over the slots of a warp, then over the four warps
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float x = l[nt][i];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (g == 0) {
+                    float* st = s_stat[warp][8 * nt + 2 * t + i];
+                    st[0] = m[nt][i];
+                    st[1] = my[nt][i];
+                    st[2] = x;
+                }
+            }
+        __syncthreads();  // statistics are there; every warp is done with its ring
+        float* s_o = reinterpret_cast<float*>(q8_smem);  // [warp][row][128]
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int d = 0; d < 8; ++d)
+                    *reinterpret_cast<float2*>(s_o + (warp * 8 * NT + 8 * nt + 2 * t + i) * kHeadDim +
+                                               16 * d + 2 * g) =
+                        make_float2(o[d][nt][i], o[d][nt][i + 2]);
+        __syncthreads();
+        const bool whole = c0 == 0 && c1 == n;
+        const int slot = c0 > 0 ? 0 : 1;  // the CTA's first segment can only start inside a pair,
+                                          // and only its last can end inside one
+        const int d = threadIdx.x;  // element of the head
+        for (int r = 0; r < 8 * NT; ++r) {
+            const int rr = rb * a.rows + r;
+            if (rr >= a.tokens * a.G) break;
+            float M = -INFINITY, Y = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                M = fmaxf(M, s_stat[w][r][0]);
+                Y = fmaxf(Y, s_stat[w][r][1]);
+            }
+            float L = 0.f, A = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                L += s_stat[w][r][2] * q8_weight(s_stat[w][r][0], M);
+                A += s_o[(w * 8 * NT + r) * kHeadDim + d] * q8_weight(s_stat[w][r][1], Y);
+            }
+            if (whole) {
+                const int tok = rr / a.G, hh = rr - tok * a.G;
+                const float f = Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift);
+                a.out[(((int64_t)b * a.tokens + tok) * a.hq + (int64_t)h * a.G + hh) * kHeadDim + d] =
+                    __float2bfloat16_rn(A / L * f);
+            } else {
+                float* p = a.part + (((int64_t)blockIdx.x * 2 + slot) * a.rows + r) * kQ8PartFloats;
+                p[d] = A;
+                if (d == 0) {
+                    p[kHeadDim] = M;
+                    p[kHeadDim + 1] = Y;
+                    p[kHeadDim + 2] = L;
+                }
+            }
+        }
+        __syncthreads();  // the ring and the statistics may be written again
+        u = p0 + c1;
+    }
+}
+
+// One CTA per (sequence, query row): adds the parts of a pair that several CTAs share, in
+// order of their slots, and writes the zeros of idle sequences.
+__global__ void __launch_bounds__(kHeadDim) q8_merge_kernel(const Q8AttnArgs a) {
+    __shared__ int s_end[NK_Q8_MAX_BATCH];
+    if (threadIdx.x == 0) griddep_launch_dependents();
+    griddep_wait();
+    q8_units(a, s_end);
+    const int b = blockIdx.y;
+    const int row = blockIdx.x;                      // t * hq + head
+    const int tok = row / a.hq, head = row - tok * a.hq;
+    const int h = head / a.G, rr = tok * a.G + head - h * a.G;
+    const int rb = rr / a.rows, r = rr - rb * a.rows;
+    const int d = threadIdx.x;
+    const int per_b = a.hkv * a.row_blocks;
+    const int64_t U = (int64_t)s_end[a.batch - 1] * per_b;
+    const int n = s_end[b] - (b > 0 ? s_end[b - 1] : 0);
+    __nv_bfloat16* out = a.out + (((int64_t)b * a.tokens + tok) * a.hq + head) * kHeadDim + d;
+    if (n == 0) {
+        *out = __float2bfloat16_rn(0.f);
+        return;
+    }
+    const int G = (int)min((int64_t)a.grid, U);
+    const int64_t p0 = (b > 0 ? (int64_t)s_end[b - 1] * per_b : 0) + (int64_t)(h * a.row_blocks + rb) * n;
+    const int cf = q8_cta_of(U, G, p0), cl = q8_cta_of(U, G, p0 + n - 1);
+    if (cf == cl) return;  // written by that CTA
+    auto part = [&](int c) {  // the first CTA's part starts the pair (slot 1), the others' do not
+        return a.part + (((int64_t)c * 2 + (c == cf ? 1 : 0)) * a.rows + r) * kQ8PartFloats;
+    };
+    float M = -INFINITY, Y = -INFINITY;
+    for (int c = cf; c <= cl; ++c) {
+        const float* p = part(c);
+        M = fmaxf(M, p[kHeadDim]);
+        Y = fmaxf(Y, p[kHeadDim + 1]);
+    }
+    float L = 0.f, A = 0.f;
+    for (int c = cf; c <= cl; ++c) {
+        const float* p = part(c);
+        L += p[kHeadDim + 2] * q8_weight(p[kHeadDim], M);
+        A += p[d] * q8_weight(p[kHeadDim + 1], Y);
+    }
+    const float f = Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift);
+    *out = __float2bfloat16_rn(A / L * f);
+}
+
+static bool q8_heads_ok(int tokens, int hq, int hkv) {
+    return tokens >= 1 && tokens <= NK_Q8_MAX_TOKENS && hkv >= 1 && hq >= 1 && hq % hkv == 0 &&
+           hq / hkv <= 16 && hq <= 4096;
+}
+static bool q8_block_ok(int block) {
+    return block == 16 || block == 32 || block == 64 || block == 128;
+}
+// Query rows of one CTA: column tiles of eight, 1, 2 or 4 of them.
+static int q8_rows(int rows) { return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32); }
+
+template <int NT>
+static int q8_launch_attn(Q8AttnArgs a, cudaStream_t s) {
+    static int slots[64] = {};  // CTAs resident at once, per device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return NK_ERR_CUDA;
+    if (dev < 0 || dev >= 64) return NK_ERR_DEVICE;
+    if (slots[dev] == 0) {
+        int sms = 0, per_sm = 0;
+        if (cudaFuncSetAttribute(q8_attn_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kQ8AttnSmem) != cudaSuccess ||
+            cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, q8_attn_kernel<NT>,
+                                                          kQ8AttnThreads, kQ8AttnSmem) !=
+                cudaSuccess ||
+            per_sm < 1)
+            return NK_ERR_CUDA;
+        slots[dev] = min(sms * per_sm, kQ8MaxGrid);
+    }
+    const int64_t most = (int64_t)((a.capacity + kQ8Unit - 1) / kQ8Unit) * a.batch * a.hkv * a.row_blocks;
+    a.grid = (int)min((int64_t)slots[dev], most);
+    const int rc = launch_pdl_smem(q8_attn_kernel<NT>, dim3(a.grid), dim3(kQ8AttnThreads),
+                                   (size_t)kQ8AttnSmem, s, a);
+    if (rc != NK_OK) return rc;
+    return launch_pdl_smem(q8_merge_kernel, dim3(a.tokens * a.hq, a.batch), dim3(kHeadDim), 0, s, a);
+}
+
+}  // namespace nk
+
+extern "C" int nk_qk_norm_rope_cache_q8(const void* qkv, int64_t ld_qkv, const void* q_norm,
+                                        const void* k_norm, const void* cos_table,
+                                        const void* sin_table, const int64_t* position,
+                                        int per_sequence, void* q_out, void* k_codes,
+                                        void* v_codes, float* k_scale, float* v_scale, int batch,
+                                        int tokens, int q_heads, int kv_heads, int head_dim,
+                                        int capacity, int block, int64_t cache_batch_stride,
+                                        int64_t cache_head_stride, int64_t cache_seq_stride,
+                                        float eps, nk_stream_t stream) {
+    using namespace nk;
+    if (!qkv || !q_norm || !k_norm || !cos_table || !sin_table || !position || !q_out ||
+        !k_codes || !v_codes || !k_scale || !v_scale)
+        return NK_ERR_ARG;
+    if (head_dim != kHeadDim || batch < 1 || batch > NK_Q8_MAX_BATCH ||
+        !q8_heads_ok(tokens, q_heads, kv_heads) || capacity < 1 || capacity > kQ8MaxCapacity || tokens > capacity ||
+        !q8_block_ok(block) || ld_qkv < (int64_t)(q_heads + 2 * kv_heads) * head_dim ||
+        cache_seq_stride < head_dim)
+        return NK_ERR_SHAPE;
+    if ((((uintptr_t)qkv | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)cos_table |
+          (uintptr_t)sin_table | (uintptr_t)position | (uintptr_t)q_out) & 7u) ||
+        (((uintptr_t)k_codes | (uintptr_t)v_codes) & 15u) ||
+        (((uintptr_t)k_scale | (uintptr_t)v_scale) & 3u) || ld_qkv % 4 ||
+        cache_batch_stride % 16 || cache_head_stride % 16 || cache_seq_stride % 16)
+        return NK_ERR_ALIGN;
+    Q8AppendArgs a{};
+    a.qkv = static_cast<const __nv_bfloat16*>(qkv);
+    a.ld = ld_qkv;
+    a.qn = static_cast<const __nv_bfloat16*>(q_norm);
+    a.kn = static_cast<const __nv_bfloat16*>(k_norm);
+    a.cos_t = static_cast<const __nv_bfloat16*>(cos_table);
+    a.sin_t = static_cast<const __nv_bfloat16*>(sin_table);
+    a.position = position;
+    a.per_sequence = per_sequence != 0;
+    a.q_out = static_cast<__nv_bfloat16*>(q_out);
+    a.k = static_cast<uint8_t*>(k_codes);
+    a.v = static_cast<uint8_t*>(v_codes);
+    a.ks = k_scale;
+    a.vs = v_scale;
+    a.batch = batch;
+    a.tokens = tokens;
+    a.hq = q_heads;
+    a.hkv = kv_heads;
+    a.capacity = capacity;
+    a.block = block;
+    a.blocks = (capacity + block - 1) / block;
+    a.cb = cache_batch_stride;
+    a.ch = cache_head_stride;
+    a.cs = cache_seq_stride;
+    a.eps = eps;
+    a.q_ctas = (tokens * q_heads + kQ8Warps - 1) / kQ8Warps;
+    const int touched = (tokens + block - 2) / block + 1;  // blocks that T tokens can touch
+    return launch_pdl_smem(q8_append_kernel, dim3(a.q_ctas + kv_heads * touched, batch),
+                           dim3(32 * kQ8Warps), 0, (cudaStream_t)stream, a);
+}
+
+extern "C" size_t nk_attention_q8_ws_bytes(int tokens, int q_heads, int kv_heads) {
+    using namespace nk;
+    if (!q8_heads_ok(tokens, q_heads, kv_heads)) return 0;
+    return (size_t)kQ8MaxGrid * 2 * q8_rows(tokens * (q_heads / kv_heads)) * kQ8PartFloats *
+           sizeof(float);
+}
+
+extern "C" int nk_attention_decode_q8(const void* q, const void* k_codes, const void* v_codes,
+                                      const float* k_scale, const float* v_scale,
+                                      const int64_t* position, int per_sequence, void* out,
+                                      int batch, int tokens, int q_heads, int kv_heads,
+                                      int head_dim, int capacity, int block,
+                                      int64_t cache_batch_stride, int64_t cache_head_stride,
+                                      int64_t cache_seq_stride, float scale, void* ws,
+                                      size_t ws_bytes, nk_stream_t stream) {
+    using namespace nk;
+    if (!q || !k_codes || !v_codes || !k_scale || !v_scale || !position || !out) return NK_ERR_ARG;
+    if (head_dim != kHeadDim || batch < 1 || batch > NK_Q8_MAX_BATCH ||
+        !q8_heads_ok(tokens, q_heads, kv_heads) || capacity < 1 || capacity > kQ8MaxCapacity || tokens > capacity ||
+        !q8_block_ok(block) || cache_seq_stride < head_dim)
+        return NK_ERR_SHAPE;
+    Q8AttnArgs a{};
+    a.G = q_heads / kv_heads;
+    a.rows = q8_rows(tokens * a.G);
+    a.row_blocks = (tokens * a.G + a.rows - 1) / a.rows;
+    const int64_t most = (int64_t)((capacity + kQ8Unit - 1) / kQ8Unit) * batch;
+    if (most > (1 << 30)) return NK_ERR_SHAPE;  // running sums of units are 32-bit
+    if (!ws || ws_bytes < nk_attention_q8_ws_bytes(tokens, q_heads, kv_heads))
+        return NK_ERR_WORKSPACE;
+    if ((((uintptr_t)q | (uintptr_t)position | (uintptr_t)out) & 7u) ||
+        (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)ws) & 15u) ||
+        (((uintptr_t)k_scale | (uintptr_t)v_scale) & 3u) || cache_batch_stride % 16 ||
+        cache_head_stride % 16 || cache_seq_stride % 16)
+        return NK_ERR_ALIGN;
+    a.q = static_cast<const __nv_bfloat16*>(q);
+    a.k = static_cast<const uint8_t*>(k_codes);
+    a.v = static_cast<const uint8_t*>(v_codes);
+    a.ks = k_scale;
+    a.vs = v_scale;
+    a.position = position;
+    a.per_sequence = per_sequence != 0;
+    a.out = static_cast<__nv_bfloat16*>(out);
+    a.part = static_cast<float*>(ws);
+    a.batch = batch;
+    a.tokens = tokens;
+    a.hq = q_heads;
+    a.hkv = kv_heads;
+    a.capacity = capacity;
+    a.block = block;
+    a.blocks = (capacity + block - 1) / block;
+    a.cb = cache_batch_stride;
+    a.ch = cache_head_stride;
+    a.cs = cache_seq_stride;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    cudaStream_t s = (cudaStream_t)stream;
+    switch (a.rows) {
+        case 8: return q8_launch_attn<1>(a, s);
+        case 16: return q8_launch_attn<2>(a, s);
+        default: return q8_launch_attn<4>(a, s);
+    }
+}

@@ -7,3 +7,5 @@
 #include "nk_static.cu"
 #include "nk_decode.cu"
 #include "nk_comm.cu"
+#include "nk_w4.cu"
+#include "nk_kvq.cu"

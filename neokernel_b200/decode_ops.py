@@ -11,6 +11,15 @@ host synchronisation. Each replaces one of the reference engine's Triton wrapper
                             in one launch, qkv never stored
 * ``attention_decode``   <- ``attention_out``       (engine/kernels/attention.py:53-62)
 * ``silu_mul``           <- ``silu_mul_out``        (engine/kernels/elementwise.py:91-101)
+
+The KV cache can also be held in 8 bits (include/nk_quant.h; the reference has no such form):
+
+* ``Q8Cache``                 e4m3 keys and values with a power-of-two scale per (sequence, kv
+                              head, block of tokens)
+* ``qk_norm_rope_cache_q8``   ``qk_norm_rope_cache`` appending to a ``Q8Cache``
+* ``attention_decode_q8``     ``attention_decode`` over a ``Q8Cache``
+
+Both take per-sequence positions, idle sequences and up to 16 new tokens a sequence.
 """
 
 from __future__ import annotations
@@ -144,3 +153,193 @@ def silu_mul(gate_up: torch.Tensor, out: torch.Tensor):
                                        out.shape[1], _stream(out))
     if st != _lib.NK_OK:
         _raise(st, "nk_silu_mul_bf16")
+
+
+Q8_MAX_TOKENS = 16   # new tokens per sequence and call (NK_Q8_MAX_TOKENS)
+Q8_MAX_BATCH = 1024  # NK_Q8_MAX_BATCH
+Q8_BLOCKS = (16, 32, 64, 128)
+
+
+class Q8Cache:
+    """A layer's KV cache in 8 bits: e4m3 codes ``k``, ``v`` [batch, kv_heads, capacity, 128] and
+    fp32 scales ``k_scale``, ``v_scale`` [batch, kv_heads, ceil(capacity / block)]; the value held
+    at slot j is ``k[..., j, :] * k_scale[..., j // block]``. The codes may have any batch, head
+    and token strides that are multiples of 16, the same for ``k`` and ``v``; the scales are
+    contiguous. The tensors are the caller's and are read and written in place."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "block", "batch", "kv_heads", "capacity",
+                 "device", "_ptrs", "_dims")
+
+    def __init__(self, k, v, k_scale, v_scale, block: int):
+        for t in (k, v):
+            _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float8_e4m3fn
+                  and t.dim() == 4 and t.shape[3] == HEAD_DIM,
+                  "Q8Cache: k and v must be float8_e4m3fn CUDA tensors [batch, kv_heads, "
+                  "capacity, 128]")
+        _need(v.shape == k.shape and v.stride() == k.stride() and v.device == k.device,
+              "Q8Cache: k and v must have the same shape, strides and device")
+        _need(block in Q8_BLOCKS, f"Q8Cache: block must be one of {Q8_BLOCKS}, got {block}")
+        B, H, S, _ = k.shape
+        _need(1 <= B <= Q8_MAX_BATCH and H >= 1 and S >= 1,
+              f"Q8Cache: batch 1..{Q8_MAX_BATCH}, kv_heads >= 1 and capacity >= 1")
+        sb, sh, ss, sd = k.stride()
+        # sorted by stride, each dimension starts past the extent of the ones below it
+        extent, dense = HEAD_DIM, sd == 1
+        for st, n in sorted((st, n) for st, n in ((sb, B), (sh, H), (ss, S)) if n > 1):
+            dense = dense and st >= extent and st % 16 == 0
+            extent = st * n
+        _need(dense and k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0,
+              "Q8Cache: unsupported layout (unit stride along the head, other strides multiples "
+              "of 16 that do not overlap, 16-byte aligned)")
+        shape = (B, H, -(-S // block))
+        for t in (k_scale, v_scale):
+            _need(isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.device == k.device
+                  and tuple(t.shape) == shape and t.is_contiguous(),
+                  f"Q8Cache: scales must be contiguous fp32 {list(shape)} on the codes' device")
+        self.k, self.v, self.k_scale, self.v_scale, self.block = k, v, k_scale, v_scale, block
+        self.batch, self.kv_heads, self.capacity, self.device = B, H, S, k.device
+        self._ptrs = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        strides = (sb if B > 1 else 0, sh if H > 1 else 0, ss if S > 1 else HEAD_DIM)
+        self._dims = (HEAD_DIM, S, block, *strides)
+
+    @classmethod
+    def empty(cls, batch: int, kv_heads: int, capacity: int, device, block: int = 64,
+              layout: str = "bhsd"):
+        """A zeroed cache; ``layout`` "bhsd" keeps a head's tokens adjacent, "bshd" a token's
+        heads (the reference supports both for its bf16 cache)."""
+        _need(layout in ("bhsd", "bshd"), f"Q8Cache: layout must be bhsd or bshd, not {layout!r}")
+        _need(block in Q8_BLOCKS, f"Q8Cache: block must be one of {Q8_BLOCKS}, got {block}")
+
+        def codes():
+            shape = ((batch, kv_heads, capacity) if layout == "bhsd"
+                     else (batch, capacity, kv_heads))
+            t = torch.zeros(*shape, HEAD_DIM, dtype=torch.uint8, device=device)
+            return (t if layout == "bhsd" else t.transpose(1, 2)).view(torch.float8_e4m3fn)
+
+        def scales():
+            return torch.zeros(batch, kv_heads, -(-capacity // block), dtype=torch.float32,
+                               device=device)
+
+        return cls(codes(), codes(), scales(), scales(), block)
+
+    def zero_(self):
+        for t in (self.k, self.v):
+            t.view(torch.uint8).zero_()
+        self.k_scale.zero_()
+        self.v_scale.zero_()
+        return self
+
+    def dequantize(self):
+        """Keys and values, fp32 [batch, kv_heads, capacity, 128]."""
+        def full(codes, scale):
+            return codes.float() * scale.repeat_interleave(self.block, dim=2)[:, :, :self.capacity,
+                                                                              None]
+        return full(self.k, self.k_scale), full(self.v, self.v_scale)
+
+
+def _q8_rows(x, cache, width, name):
+    """(tokens per sequence, row stride) of a [batch * tokens, width] bf16 operand."""
+    _need(isinstance(x, torch.Tensor) and x.dtype is torch.bfloat16 and x.device == cache.device
+          and x.dim() == 2, f"{name} must be a 2-D bf16 tensor on the cache's device")
+    rows = x.shape[0]
+    T = rows // cache.batch
+    _need(x.shape[1] == width and T * cache.batch == rows and 1 <= T <= Q8_MAX_TOKENS
+          and T <= cache.capacity,
+          f"{name} must be [batch * tokens, {width}] for batch {cache.batch}, tokens 1.."
+          f"{Q8_MAX_TOKENS} within the capacity {cache.capacity}, got {list(x.shape)}")
+    return T
+
+
+def _q8_position(position, cache, name):
+    """1 if the int64 ``position`` has an entry per sequence, 0 if one for all."""
+    _need(isinstance(position, torch.Tensor) and position.dtype is torch.int64
+          and position.device == cache.device and position.is_contiguous()
+          and position.numel() in (1, cache.batch) and position.dim() == 1,
+          f"{name}: position must be a contiguous int64 tensor [1] or [{cache.batch}] on the "
+          "cache's device")
+    return 1 if position.numel() == cache.batch else 0
+
+
+def _on(device, fn, args):
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return fn(*args)
+    return fn(*args)
+
+
+def qk_norm_rope_cache_q8(qkv, q_norm, k_norm, cos, sin, position, q_out, cache: Q8Cache,
+                          heads: int, eps: float):
+    """``qk_norm_rope_cache`` for T = 1..16 new tokens per sequence, appending to a ``Q8Cache``.
+
+    qkv [batch * T, (heads + 2 kv_heads) * 128] (row b * T + t, unit column stride); ``position``
+    [batch] (or [1], shared): slot of each sequence's first new token, negative for an idle
+    sequence, of which nothing is read or written. q_out [batch * T, heads * 128] contiguous. A
+    block's scale is the smallest power of two that keeps its new tokens within e4m3's range,
+    and at least its former one where it holds earlier tokens; these are rounded anew when it
+    rises. A position past capacity - T is an idle sequence too and is reported by ``device_error()``."""
+    name = "qk_norm_rope_cache_q8"
+    H, Hkv = int(heads), cache.kv_heads
+    _need(H >= 1 and H % Hkv == 0, f"{name}: heads must be a multiple of the cache's {Hkv}")
+    T = _q8_rows(qkv, cache, (H + 2 * Hkv) * HEAD_DIM, f"{name}: qkv")
+    _need(_q8_rows(q_out, cache, H * HEAD_DIM, f"{name}: q_out") == T and q_out.is_contiguous(),
+          f"{name}: q_out must be contiguous, with as many rows as qkv")
+    per = _q8_position(position, cache, name)
+    st = qkv.stride()
+    ld = st[0] if qkv.shape[0] > 1 else qkv.shape[1]
+    _need(st[1] == 1 and ld >= qkv.shape[1] and ld % 4 == 0 and qkv.data_ptr() % 8 == 0
+          and q_out.data_ptr() % 8 == 0,
+          f"{name}: qkv rows must have unit column stride, 8-byte aligned")
+    for t, shape in ((q_norm, (HEAD_DIM,)), (k_norm, (HEAD_DIM,))):
+        _need(isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.shape == shape
+              and t.device == cache.device and t.stride(0) == 1 and t.data_ptr() % 8 == 0,
+              f"{name}: q_norm and k_norm must be bf16 [128] on the cache's device")
+    for t in (cos, sin):
+        _need(isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.dim() == 2
+              and t.shape[0] >= cache.capacity and t.shape[1] == HEAD_DIM and t.is_contiguous()
+              and t.device == cache.device and t.data_ptr() % 8 == 0,
+              f"{name}: cos and sin must be contiguous bf16 [capacity, 128] on the cache's device")
+    status = _on(cache.device, _lib.load().nk_qk_norm_rope_cache_q8, (
+        qkv.data_ptr(), ld, q_norm.data_ptr(), k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+        position.data_ptr(), per, q_out.data_ptr(), *cache._ptrs, cache.batch, T, H, Hkv,
+        *cache._dims, float(eps), _stream(qkv)))
+    if status != _lib.NK_OK:
+        _raise(status, "nk_qk_norm_rope_cache_q8")
+    return q_out
+
+
+def attention_q8_workspace(cache: Q8Cache, heads: int, tokens: int = 1) -> torch.Tensor:
+    """Workspace of ``attention_decode_q8`` for up to ``tokens`` new tokens per sequence, on the
+    cache's device. Its size does not depend on the batch or the capacity, so the layers of a
+    model, whose calls are ordered, share one. Two streams (or graphs) that may run at once need
+    one each."""
+    n = int(_lib.load().nk_attention_q8_ws_bytes(tokens, heads, cache.kv_heads))
+    _need(n > 0, f"attention_q8_workspace: tokens 1..{Q8_MAX_TOKENS}, heads 1..16 times "
+                 f"{cache.kv_heads}; got tokens={tokens}, heads={heads}")
+    return torch.empty(n, dtype=torch.uint8, device=cache.device)
+
+
+def attention_decode_q8(q, cache: Q8Cache, position, out, ws, heads: int,
+                        scale: float | None = None):
+    """``attention_decode`` of T = 1..16 new tokens per sequence over a ``Q8Cache`` that already
+    holds them: row b * T + t of q, out [batch * T, heads * 128] attends over slots
+    [0, position[b] + t]. ``position`` as in ``qk_norm_rope_cache_q8``; rows of idle sequences
+    come out zero. ``heads`` is 1 to 16 times the cache's kv_heads."""
+    name = "attention_decode_q8"
+    H = int(heads)
+    _need(H >= 1 and H % cache.kv_heads == 0 and H // cache.kv_heads <= 16,
+          f"{name}: heads must be 1 to 16 times the cache's {cache.kv_heads}")
+    T = _q8_rows(q, cache, H * HEAD_DIM, f"{name}: q")
+    _need(_q8_rows(out, cache, H * HEAD_DIM, f"{name}: out") == T and q.is_contiguous()
+          and out.is_contiguous() and q.data_ptr() % 8 == 0 and out.data_ptr() % 8 == 0,
+          f"{name}: q and out must be contiguous, 8-byte aligned and of the same shape")
+    per = _q8_position(position, cache, name)
+    _need(isinstance(ws, torch.Tensor) and ws.device == cache.device and ws.is_contiguous(),
+          f"{name}: ws must be a workspace on the cache's device")
+    scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
+    status = _on(cache.device, _lib.load().nk_attention_decode_q8, (
+        q.data_ptr(), *cache._ptrs, position.data_ptr(), per, out.data_ptr(), cache.batch, T, H,
+        cache.kv_heads, *cache._dims, scale, ws.data_ptr(), ws.numel() * ws.element_size(),
+        _stream(q)))
+    if status != _lib.NK_OK:
+        _raise(status, "nk_attention_decode_q8")
+    return out

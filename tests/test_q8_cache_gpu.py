@@ -1,0 +1,435 @@
+"""The 8-bit KV cache (neokernel_b200.decode_ops: Q8Cache, qk_norm_rope_cache_q8,
+attention_decode_q8) against plain implementations in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+import neokernel_b200 as nk
+from neokernel_b200 import _lib, decode_ops as ops, qwen3
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+EPS = 1e-6
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def rand(*shape, std=1.0, seed=0):
+    return (torch.randn(shape, generator=gen(seed), device=DEV) * std).to(torch.bfloat16)
+
+
+def filled_cache(B, H, S, block, layout="bhsd", seed=0, lo=-9, hi=-4):
+    c = ops.Q8Cache.empty(B, H, S, DEV, block=block, layout=layout)
+    for n, t in ((0, c.k), (1, c.v)):
+        x = torch.randn(t.shape, generator=gen(seed + n), device=DEV).mul_(80).clamp_(-448, 448)
+        t.view(torch.uint8).copy_(x.to(torch.float8_e4m3fn).view(torch.uint8))
+    for n, t in ((2, c.k_scale), (3, c.v_scale)):
+        t.copy_(torch.exp2(torch.randint(lo, hi, t.shape, generator=gen(seed + n), device=DEV).float()))
+    return c
+
+
+def poison(cache, first_free):
+    """Codes of NaN and scales of NaN from slot first_free[b] on (scales: of whole free blocks)."""
+    for b, n in enumerate(first_free):
+        for t in (cache.k, cache.v):
+            t.view(torch.uint8)[b, :, n:] = 0x7f
+        for t in (cache.k_scale, cache.v_scale):
+            t[b, :, -(-n // cache.block):] = float("nan")
+
+
+# ---------------------------------------------------------------------------- attention
+def attention_ref(q, cache, pos, heads, scale=None):
+    """(out, tolerance) in 64 bits. Errors: a score's fp32 sum of 128 exact products in 8 matrix
+    instructions, at most 128 + 8 additions and 4 products each off by 2^-23 of sum |q k|; an
+    exponential off by the score's error times ln 2 plus 2^-21 (exp2f and the argument's
+    rounding at magnitudes to 2^7: 2^-17); a probability rounded to f16 (2^-11); fp32 sums over the
+    slots, at most len additions of 2^-23; the bf16 rounding of the result."""
+    B, T, Hkv = cache.batch, q.shape[0] // cache.batch, cache.kv_heads
+    G = heads // Hkv
+    scale = 1 / math.sqrt(128) if scale is None else scale
+    out = torch.zeros(B, T, heads, 128, device=DEV, dtype=torch.float64)
+    tol = torch.zeros_like(out)
+    qd = q.view(B, T, heads, 128).double()
+    for b in range(B):
+        p0 = pos[b]
+        if p0 < 0 or p0 > cache.capacity - T:
+            continue
+        n = p0 + T
+        k, v = (t[b, :, :n].double() * s[b].double().repeat_interleave(cache.block, 1)[:, :n, None]
+                for t, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+        for h in range(Hkv):
+            hs = slice(h * G, h * G + G)
+            x = torch.einsum("tgd,sd->tgs", qd[b, :, hs], k[h]) * scale
+            seen = torch.arange(n, device=DEV)[None, None] <= (p0 + torch.arange(T, device=DEV))[:, None, None]
+            w = torch.softmax(x.masked_fill(~seen, float("-inf")), dim=-1)
+            o = w @ v[h]
+            mag = torch.einsum("tgd,sd->tgs", qd[b, :, hs].abs(), k[h].abs()) * scale
+            err = 140 * 2.0 ** -23 * (mag * seen).amax(-1, keepdim=True) + 2.0 ** -17
+            rel = 2 * err + 2.0 ** -11 + (n + 64) * 2.0 ** -23
+            out[b, :, hs] = o
+            tol[b, :, hs] = torch.finfo(torch.bfloat16).eps / 2 * o.abs() + rel * (w @ v[h].abs())
+    return out.view(B * T, -1), tol.view(B * T, -1)
+
+
+def run_attention(q, cache, pos, heads, scale=None, out=None):
+    T = q.shape[0] // cache.batch
+    ws = ops.attention_q8_workspace(cache, heads, T)
+    ws.fill_(0xff)
+    out = torch.full_like(q, float("nan")) if out is None else out
+    position = torch.tensor(pos, device=DEV)
+    assert ops.attention_decode_q8(q, cache, position, out, ws, heads, scale) is out
+    return out
+
+
+def check_attention(q, cache, pos, heads, scale=None):
+    full = pos if len(pos) == cache.batch else pos * cache.batch
+    out = run_attention(q, cache, pos, heads, scale)
+    ref, tol = attention_ref(q, cache, full, heads, scale)
+    # a NaN among the codes (values past 448 become one) makes the formula's row NaN too
+    bad = ~(((out.double() - ref).abs() <= tol) | (out.isnan() & ref.isnan()))
+    assert not bad.any(), (f"{int(bad.sum())} of {bad.numel()} off, worst "
+                           f"{((out.double() - ref).abs() / tol.clamp_min(1e-30)).max().item()} tol")
+    return out
+
+
+@pytest.mark.parametrize("heads,kv", [(32, 8), (64, 8), (8, 8), (4, 1), (5, 1), (28, 4), (16, 1)])
+@pytest.mark.parametrize("T", (1, 2, 5, 16))
+def test_attention_heads_and_tokens(heads, kv, T):
+    S = 300
+    cache = filled_cache(3, kv, S, 64, seed=heads + T)
+    pos = [0, 131, S - T]
+    poison(cache, [p + T for p in pos])
+    check_attention(rand(3 * T, heads * 128, seed=T), cache, pos, heads)
+
+
+@pytest.mark.parametrize("block", (16, 32, 64, 128))
+@pytest.mark.parametrize("layout", ("bhsd", "bshd"))
+@pytest.mark.parametrize("S", (1, 16, 17, 63, 64, 65, 129, 1000))
+def test_attention_lengths(block, layout, S):
+    cache = filled_cache(2, 2, S, block, layout, seed=S)
+    for pos in sorted({0, S // 2, max(0, S - 2), S - 1}):
+        poison(cache, [pos + 1, S])
+        check_attention(rand(2, 8 * 128, seed=pos), cache, [pos, S - 1], 8)
+        cache = filled_cache(2, 2, S, block, layout, seed=S)
+
+
+@pytest.mark.parametrize("B,S", [(1, 8192), (40, 700), (7, 5000)])
+def test_attention_ragged_batches(B, S):
+    """Lengths from nothing to everything; an idle sequence's rows come out zero."""
+    cache = filled_cache(B, 8, S, 64, seed=B)
+    pos = [(S - 1) * (b + 1) // B for b in range(B)]
+    if B > 2:
+        pos[1] = -1
+        pos[B // 2] = 0
+    poison(cache, [p + 1 if p >= 0 else 0 for p in pos])
+    out = check_attention(rand(B, 32 * 128, seed=B), cache, pos, 32)
+    if B > 2:
+        assert (out[1] == 0).all()
+    assert nk.device_error() == 0
+
+
+def test_attention_shared_position_and_scale():
+    cache = filled_cache(4, 8, 512, 32, seed=3)
+    q = rand(4, 32 * 128, seed=4)
+    shared = check_attention(q, cache, [300], 32, scale=0.3)
+    each = run_attention(q, cache, [300] * 4, 32, scale=0.3)
+    assert torch.equal(shared, each)
+
+
+def test_attention_all_idle_and_out_of_range():
+    cache = filled_cache(3, 2, 64, 16)
+    poison(cache, [0, 0, 0])
+    q = rand(3, 4 * 128)
+    assert (run_attention(q, cache, [-1, -5, -2 ** 62], 4) == 0).all()
+    assert nk.device_error() == 0
+    assert (run_attention(q, cache, [64, -1, 2 ** 62], 4) == 0).all()
+    assert nk.device_error() == _lib.NK_ERR_RANGE
+    assert nk.device_error() == 0
+
+
+def test_attention_value_scales_far_apart():
+    """Blocks whose values differ by 2^90, with a peaked softmax on either end."""
+    cache = filled_cache(1, 1, 256, 16, seed=5)
+    cache.v_scale[0, 0] = torch.exp2(torch.linspace(-60, 30, 16, device=DEV).round())
+    for target in (3, 250):
+        q = (cache.k[0, 0, target].float() * 0.05).to(torch.bfloat16).view(1, 128)
+        cache.k_scale.fill_(2.0 ** -3)
+        check_attention(q, cache, [255], 1)
+
+
+def test_attention_zero_scales_and_flat_scores():
+    cache = filled_cache(2, 2, 200, 32, seed=6)
+    cache.k_scale.zero_()          # every score 0: a mean of the values
+    cache.v_scale[1].zero_()       # and values of 0
+    out = check_attention(rand(2, 4 * 128, seed=2), cache, [199, 150], 4)
+    assert (out[1] == 0).all()
+
+
+@pytest.mark.parametrize("where", ("k", "v", "q"))
+def test_attention_nan_is_not_lost(where):
+    cache = filled_cache(2, 2, 400, 64, seed=7)
+    q = rand(2, 4 * 128, seed=3)
+    clean = run_attention(q, cache, [399, 399], 4)
+    if where == "q":
+        q[1, 5] = float("nan")
+    else:
+        getattr(cache, where).view(torch.uint8)[1, 0, 100:164, 7 if where == "v" else slice(None)] = 0x7f
+    out = run_attention(q, cache, [399, 399], 4)
+    assert torch.equal(out[0], clean[0])
+    row, before = out[1].view(4, 128), clean[1].view(4, 128)
+    if where == "q":
+        assert row[0].isnan().all() and torch.equal(row[1:], before[1:])
+    elif where == "k":
+        assert row[:2].isnan().all() and torch.equal(row[2:], before[2:])
+    else:
+        assert row[:2, 7].isnan().all() and torch.equal(row[2:], before[2:])
+        assert torch.equal(row[:2, :7], before[:2, :7])
+
+
+def test_attention_large_and_tiny_queries():
+    cache = filled_cache(1, 1, 128, 64, seed=8)
+    for std in (1e-30, 1e-4, 30.0):
+        check_attention(rand(1, 2 * 128, std=std, seed=9), cache, [127], 2)
+
+
+def test_attention_past_32_bit_offsets():
+    """A cache of 4.5 GB of keys: the last sequence's codes start past 2^32."""
+    B, H, S = 9, 8, 1 << 19
+    k = torch.zeros(B, H, S, 128, dtype=torch.uint8, device=DEV)
+    v = torch.zeros_like(k)
+    s = torch.full((B, H, S // 128), 2.0 ** -6, device=DEV)
+    for t in (k, v):
+        x = torch.randn(H, 2000, 128, generator=gen(1), device=DEV).mul_(80)
+        t[-1, :, :2000] = x.to(torch.float8_e4m3fn).view(torch.uint8)
+    cache = ops.Q8Cache(k.view(torch.float8_e4m3fn), v.view(torch.float8_e4m3fn), s, s.clone(), 128)
+    pos = [-1] * (B - 1) + [1999]
+    check_attention(rand(B, 8 * 128, seed=1), cache, pos, 8)
+
+
+def test_attention_same_bits_and_captured():
+    cache = filled_cache(6, 8, 3000, 64, seed=10)
+    q = rand(6, 32 * 128, seed=11)
+    pos = [5, 2999, 1000, -1, 64, 2000]
+    a, b = run_attention(q, cache, pos, 32), run_attention(q, cache, pos, 32)
+    assert torch.equal(a, b)
+    # captured at one set of lengths, replayed at others; two graphs with a workspace each
+    position = torch.zeros(6, dtype=torch.int64, device=DEV)
+    graphs, outs = [], []
+    for _ in range(2):
+        ws, out = ops.attention_q8_workspace(cache, 32), torch.empty_like(q)
+        g = torch.cuda.CUDAGraph()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(g, stream=s):
+            ops.attention_decode_q8(q, cache, position, out, ws, 32)
+        graphs.append((g, ws, s))
+        outs.append(out)
+    position.copy_(torch.tensor(pos, device=DEV))
+    torch.cuda.synchronize()
+    for g, _, s in graphs:
+        with torch.cuda.stream(s):
+            g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], a) and torch.equal(outs[1], a)
+
+
+# ---------------------------------------------------------------------------- append
+def e4m3(x):
+    """Nearest e4m3 value of fp64 x, ties to even."""
+    _, e = torch.frexp(x)
+    step = torch.exp2((e - 1).clamp(min=-6).double() - 3)
+    return torch.round(x / step) * step
+
+
+def scale_of(amax):
+    if amax == 0:
+        return 0.0
+    return 2.0 ** max(-64, math.ceil(math.log2(amax / 448.0)))
+
+
+def rows_ref(x, gain, cos, sin):
+    """RMSNorm + RoPE with the step's bf16 cast points, in 64 bits between them; x [..., 128]."""
+    r = lambda t: t.to(torch.bfloat16).double()  # noqa: E731
+    n = r(r(x / torch.sqrt(x.square().mean(-1, keepdim=True) + EPS)) * gain.double())
+    rot = torch.cat((-n[..., 64:], n[..., :64]), dim=-1)
+    return r(r(n * cos) + r(rot * sin))
+
+
+def tables(S):
+    return qwen3.rope_tables(qwen3.Qwen3Dims(1024, 1024, 8, 8, 128, 1, 64), S, DEV)
+
+
+def append(cache, qkv, heads, pos, cos, sin, qn, kn):
+    q_out = torch.full((qkv.shape[0], heads * 128), 3.0, dtype=torch.bfloat16, device=DEV)
+    assert ops.qk_norm_rope_cache_q8(qkv, qn, kn, cos, sin, torch.tensor(pos, device=DEV), q_out,
+                                     cache, heads, EPS) is q_out
+    return q_out
+
+
+def check_append(cache, qkv, heads, pos, T):
+    """Scales and value codes exactly; queries and key codes as the cast points leave them, save
+    that a value whose fp32 norm falls on the other side of a bf16 rounding border (2^-24 errors
+    on steps of 2^-8: one in thousands) moves by one bf16 step (2^-7), and its code by one
+    e4m3 step (2^-3 of it)."""
+    B, H, S, block = cache.batch, cache.kv_heads, cache.capacity, cache.block
+    cos, sin = tables(S)
+    qn, kn = (torch.rand(128, generator=gen(i), device=DEV) + 0.5 for i in (50, 51))
+    qn, kn = qn.to(torch.bfloat16), kn.to(torch.bfloat16)
+    before = [t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    q_out = append(cache, qkv, heads, pos, cos, sin, qn, kn)
+    rows = qkv.view(B, T, heads + 2 * H, 128).double()
+    for b in range(B):
+        p = pos[b if len(pos) > 1 else 0]
+        if p < 0 or p > S - T:
+            assert (q_out[b * T:b * T + T] == 3.0).all()
+            for t, t0 in zip((cache.k, cache.v), before):
+                assert torch.equal(t[b].view(torch.uint8), t0[b].view(torch.uint8))
+            for t, t0 in zip((cache.k_scale, cache.v_scale), before[2:]):
+                assert torch.equal(t[b], t0[b], )
+            continue
+        c, s = (t[p:p + T].double()[:, None] for t in (cos, sin))
+        want_q = rows_ref(rows[b, :, :heads], qn, c, s).view(T, -1)
+        got_q = q_out[b * T:b * T + T].double()
+        assert ((got_q - want_q).abs() <= 2.0 ** -7 * want_q.abs() + 2.0 ** -7 * 4).all()
+        assert (got_q == want_q).double().mean() > 0.99
+        new = (rows_ref(rows[b, :, heads:heads + H], kn, c, s), rows[b, :, heads + H:])
+        for i, (code, scale) in enumerate(((cache.k, cache.k_scale), (cache.v, cache.v_scale))):
+            code0, scale0 = before[i][b], before[2 + i][b]
+            want, want_s = code0.double(), scale0.clone()
+            for j in range(p // block, (p + T - 1) // block + 1):
+                lo, hi = max(p, j * block), min(p + T, j * block + block)
+                for h in range(H):
+                    x = new[i][lo - p:hi - p, h]
+                    fin = x[x.isfinite()]
+                    sc = scale_of(fin.abs().max().item() if fin.numel() else 0.0)
+                    if lo > j * block:
+                        sc = max(sc, scale0[h, j].item())
+                        old = code0[h, j * block:lo].double()
+                        want[h, j * block:lo] = e4m3(old * (scale0[h, j].item() / sc)) if sc else old
+                    want_s[h, j] = sc
+                    q8 = e4m3(x / sc) if sc else torch.zeros_like(x)
+                    want[h, lo:hi] = torch.where(x.isfinite(), q8, torch.full_like(x, float("nan")))
+            assert torch.equal(scale[b], want_s)
+            got = code[b].double()
+            same = (got == want) | (got.isnan() & want.isnan())
+            if i == 1:
+                assert same.all()
+            else:
+                near = (got - want).abs() <= 2.0 ** -3 * want.abs() + 2.0 ** -9
+                assert (same | near).all() and same.double().mean() > 0.99
+
+
+@pytest.mark.parametrize("block", (16, 32, 64, 128))
+@pytest.mark.parametrize("layout", ("bhsd", "bshd"))
+@pytest.mark.parametrize("T", (1, 3, 16))
+def test_append(block, layout, T):
+    S = 200
+    for seed, pos in enumerate(([0, 1, 15, 16], [63, 64, 100, S - T], [127 - T, 128 - T, -1, 31])):
+        cache = filled_cache(4, 2, S, block, layout, seed=seed)
+        qkv = rand(4 * T, 8 * 128, seed=10 + seed)
+        check_append(cache, qkv, 4, pos, T)
+    assert nk.device_error() == 0
+
+
+@pytest.mark.parametrize("heads,kv", [(32, 8), (64, 8), (8, 8), (5, 1), (3, 3)])
+def test_append_heads(heads, kv):
+    cache = filled_cache(2, kv, 64, 16, seed=kv)
+    check_append(cache, rand(2 * 2, (heads + 2 * kv) * 128, seed=heads), heads, [30], 2)
+
+
+def test_append_rises_and_stays():
+    """A block's scale rises with a larger token (earlier codes are rounded anew) and does not
+    fall with smaller ones; the first token of a block ignores what the block held before."""
+    cache = filled_cache(1, 1, 64, 16, seed=1, lo=20, hi=21)
+    for p, std in ((16, 1e-3), (17, 1.0), (18, 1e-4), (19, 3e4), (20, 0.0), (32, 0.0), (33, 1e-20)):
+        check_append(cache, rand(1, 3 * 128, std=std, seed=p), 1, [p], 1)
+
+
+def test_append_extremes():
+    """Zeros, the largest bf16 values, values below the least scale, and values that are not
+    finite (stored as NaN, the block's scale from the others)."""
+    qkv = rand(4, 3 * 128, seed=2)
+    qkv[0, 256:] = 0.0
+    qkv[1, 256:300] = torch.finfo(torch.bfloat16).max
+    qkv[2, 256:] = 2.0 ** -100
+    qkv[3, 256] = float("inf")
+    qkv[3, 257] = float("nan")
+    for p in (0, 5):
+        check_append(filled_cache(1, 1, 32, 16, seed=4), qkv, 1, [p], 4)
+        check_append(filled_cache(4, 1, 32, 16, seed=5), qkv, 1, [p], 1)
+
+
+def test_append_out_of_range_and_strided_rows():
+    cache = filled_cache(3, 2, 40, 16, seed=6)
+    wide = rand(3, 8 * 128 + 12, seed=7)
+    check_append(cache, wide[:, 4:4 + 8 * 128].contiguous(), 4, [40, 39, -7], 1)
+    assert nk.device_error() == _lib.NK_ERR_RANGE
+    a, b = filled_cache(3, 2, 40, 16, seed=6), filled_cache(3, 2, 40, 16, seed=6)
+    cos, sin = tables(40)
+    qn = kn = torch.ones(128, dtype=torch.bfloat16, device=DEV)
+    qa = append(a, wide[:, 4:4 + 8 * 128], 4, [3, 4, 5], cos, sin, qn, kn)
+    qb = append(b, wide[:, 4:4 + 8 * 128].contiguous(), 4, [3, 4, 5], cos, sin, qn, kn)
+    assert torch.equal(qa, qb)
+    assert torch.equal(a.k.view(torch.uint8), b.k.view(torch.uint8))
+
+
+def test_append_then_attend():
+    """Tokens appended one by one, in drafts and all at once, then attended: the attention of
+    what the cache stands for, close to that of the unrounded keys and values."""
+    B, heads, kv, S = 2, 8, 2, 96
+    cos, sin = tables(S)
+    qn = kn = torch.ones(128, dtype=torch.bfloat16, device=DEV)
+    qkv = rand(B * 48, (heads + 2 * kv) * 128, seed=8).view(B, 48, -1)
+    for T in (1, 4, 16):
+        cache = ops.Q8Cache.empty(B, kv, S, DEV, block=16)
+        poison(cache, [0, 0])
+        for p in range(0, 48, T):
+            x = qkv[:, p:p + T].reshape(B * T, -1)
+            q = append(cache, x, heads, [p, p], cos, sin, qn, kn)
+            out = check_attention(q, cache, [p, p], heads)
+        k, v = cache.dequantize()
+        want = qkv.view(B, 48, heads + 2 * kv, 128)[:, :, heads + kv:].transpose(1, 2).float()
+        # a code is off by half a step (2^-4) of the value or of the least normal code, and by a
+        # whole one more where the block's scale rose later
+        tol = 2.0 ** -3 * want.abs() + 2.0 ** -8 * cache.v_scale[:, :, :3].repeat_interleave(16, 2)[..., None]
+        assert ((v[:, :, :48] - want).abs() <= tol).all()
+        assert out.isfinite().all()
+
+
+def test_refusals():
+    cache = filled_cache(2, 2, 64, 16)
+    q = rand(2, 4 * 128)
+    out = torch.empty_like(q)
+    ws = ops.attention_q8_workspace(cache, 4)
+    pos = torch.zeros(2, dtype=torch.int64, device=DEV)
+    ok = dict(q=q, cache=cache, position=pos, out=out, ws=ws, heads=4)
+    for bad in (dict(heads=3), dict(heads=34), dict(q=q.float()), dict(q=q[:1]), dict(out=out[:1]),
+                dict(q=q.cpu()), dict(position=pos.int()), dict(position=pos.cpu()),
+                dict(position=torch.zeros(3, dtype=torch.int64, device=DEV)),
+                dict(ws=ws[:16]), dict(ws=ws.cpu()),
+                dict(q=rand(34, 512), out=rand(34, 512)),
+                dict(q=rand(2, 1024)[:, ::2], out=out)):
+        with pytest.raises(ValueError):
+            ops.attention_decode_q8(**(ok | bad))
+    with pytest.raises(ValueError):
+        ops.attention_q8_workspace(cache, 3)
+    cos, sin = tables(64)
+    gain = torch.ones(128, dtype=torch.bfloat16, device=DEV)
+    ok = dict(qkv=rand(2, 8 * 128), q_norm=gain, k_norm=gain, cos=cos, sin=sin, position=pos,
+              q_out=out, cache=cache, heads=4, eps=EPS)
+    for bad in (dict(heads=5), dict(qkv=rand(2, 7 * 128)), dict(qkv=rand(4, 8 * 128)),
+                dict(cos=cos[:63]), dict(sin=sin.float()), dict(q_norm=gain[:64]),
+                dict(q_out=out.float()), dict(position=pos[:0]), dict(qkv=rand(2, 8 * 128).cpu())):
+        with pytest.raises(ValueError):
+            ops.qk_norm_rope_cache_q8(**(ok | bad))
+    k, s = cache.k, cache.k_scale
+    for args in ((k, cache.v, s, s[:, :, :1], 16), (k, cache.v[:1], s, s, 16),
+                 (k.view(torch.uint8), cache.v, s, s, 16), (k, cache.v, s.double(), s, 16),
+                 (k[:, :1].expand(2, 2, 64, 128), cache.v[:, :1].expand(2, 2, 64, 128), s, s, 16),
+                 (k, cache.v, s, s, 32)):
+        with pytest.raises(ValueError):
+            ops.Q8Cache(*args)

@@ -1,0 +1,183 @@
+"""4-bit weights and the 8-bit cache without a GPU: storage layout against its description in
+include/nk_quant.h, and what the entry points refuse before any launch."""
+
+import ctypes
+
+import pytest
+import torch
+
+import neokernel_b200 as nk
+from neokernel_b200 import _lib, decode_ops as ops
+
+
+def random_w4(N, K, group, zeros, dtype=torch.bfloat16, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    G = -(-K // group)
+    q = torch.randint(0, 256, (N, -(-K // 2)), generator=g, dtype=torch.uint8)
+    s = torch.rand(N, G, generator=g).to(dtype)
+    z = torch.randint(0, 16, (N, G), generator=g, dtype=torch.uint8) if zeros else None
+    return q, s, z
+
+
+@pytest.mark.parametrize("N,K,group,zeros", [(1, 1, 32, True), (16, 128, 128, False),
+                                             (17, 129, 64, True), (40, 300, 32, True),
+                                             (33, 257, 128, True)])
+def test_storage_layout(N, K, group, zeros):
+    q, s, z = random_w4(N, K, group, zeros)
+    w = nk.W4Weight.pack(q, s, z, K=K, group=group)
+    L = _lib.load()
+    assert w.codes.nbytes == L.nk_w4_code_bytes(N, K)
+    assert w.scales.nbytes == L.nk_w4_scale_bytes(N, K, group)
+    if zeros:
+        assert w.zeros.nbytes == L.nk_w4_zero_bytes(N, K, group)
+    NB, KB, GP = -(-N // 16), -(-K // 128), -(-K // 128) * 128 // group
+    words = w.codes.view(torch.int32).view(NB, KB, 2, 32, 4)
+    scales, zp = w.scales.view(NB, GP, 8, 2), w.zeros.view(NB, GP, 8, 2) if zeros else None
+    for n in range(NB * 16):
+        i, half, r = n // 16, n % 16 // 8, n % 8
+        for k in range(0, KB * 128, 7):
+            b, j, quarter, e = k // 128, k % 128 // 32, k % 32 // 8, k % 8
+            word = int(words[i, b, half, 4 * r + quarter, j]) & 0xffffffff
+            code = word >> (4 * (e // 2) + 16 * (e % 2)) & 15
+            if n < N and k < K:
+                assert code == int(q[n, k // 2]) >> 4 * (k % 2) & 15
+                assert scales[i, k // group, r, half] == s[n, k // group]
+                if zeros:
+                    assert zp[i, k // group, r, half] == z[n, k // group]
+            else:
+                assert code == 0
+                if n >= N or k // group >= s.shape[1]:
+                    assert scales[i, k // group, r, half] == 0
+
+
+@pytest.mark.parametrize("zeros", (False, True))
+@pytest.mark.parametrize("N,K,group", [(5, 77, 32), (48, 384, 128)])
+def test_dequantize_is_the_formula(N, K, group, zeros):
+    q, s, z = random_w4(N, K, group, zeros, torch.float16)
+    w = nk.W4Weight.pack(q, s, z, K=K, group=group)
+    codes = torch.stack((q & 15, q >> 4), dim=-1).reshape(N, -1)[:, :K].float()
+    at = torch.arange(K) // group
+    want = (codes - (z.float()[:, at] if zeros else 8.0)) * s.float()[:, at]
+    assert torch.equal(w.dequantize(), want)
+    assert w.shape == (K, N)
+
+
+def test_quantize_of_zeros_and_exact_codes():
+    w = nk.W4Weight.quantize(torch.zeros(3, 64), 32)
+    assert torch.equal(w.dequantize(), torch.zeros(3, 64))
+    exact = torch.randint(-7, 8, (4, 128)).float()
+    exact[:, 0] = 7.0
+    assert torch.equal(nk.W4Weight.quantize(exact * 0.5, 128).dequantize(), exact * 0.5)
+
+
+def test_pack_refuses():
+    q, s, z = random_w4(8, 64, 32, True)
+    ok = dict(q=q, scales=s, zeros=z, K=64, group=32)
+    for bad in (dict(group=16), dict(group=48), dict(q=q.int()), dict(q=q[0]), dict(K=66),
+                dict(scales=s.float()), dict(scales=s[:, :1]), dict(zeros=z.int()),
+                dict(zeros=z[:4]), dict(zeros=torch.full_like(z, 16)), dict(K=0)):
+        with pytest.raises(ValueError):
+            nk.W4Weight.pack(**(ok | bad))
+    with pytest.raises(ValueError):
+        nk.W4Weight.quantize(torch.zeros(3, 64), 16)
+    with pytest.raises(ValueError):
+        nk.W4Weight.quantize(torch.zeros(3, 64, dtype=torch.int32))
+    w = nk.W4Weight.pack(**ok)  # on the CPU: a linear needs it on the GPU
+    with pytest.raises(ValueError):
+        nk.mm_w4(torch.zeros(1, 64, dtype=torch.bfloat16), w,
+                 out=torch.zeros(1, 8, dtype=torch.bfloat16))
+
+
+def test_w4_sizes_out_of_range():
+    L = _lib.load()
+    assert L.nk_w4_code_bytes(0, 128) == 0 and L.nk_w4_code_bytes(16, 0) == 0
+    assert L.nk_w4_scale_bytes(16, 128, 16) == 0 and L.nk_w4_scale_bytes(16, 128, 0) == 0
+    assert L.nk_w4_code_bytes((1 << 24) + 1, 128) == 0
+
+
+def test_gemm_w4_abi_refusals():
+    L = _lib.load()
+    p = ctypes.c_void_p(1 << 20)  # aligned and never read: every call is refused
+
+    def call(x=p, ldx=256, codes=p, scales=p, zeros=None, y=p, ldy=64, M=1, N=64, K=256, group=128,
+             st=0):
+        return L.nk_gemm_w4(x, ldx, codes, scales, zeros, y, ldy, M, N, K, group, st, None)
+
+    at = lambda n: ctypes.c_void_p((1 << 20) + n)  # noqa: E731
+    for kw in (dict(x=None), dict(codes=None), dict(scales=None), dict(y=None), dict(st=2),
+               dict(st=-1)):
+        assert call(**kw) == _lib.NK_ERR_ARG, kw
+    for kw in (dict(M=0), dict(M=-1), dict(M=(1 << 20) + 1), dict(N=0), dict(K=0), dict(group=16),
+               dict(group=0), dict(ldx=255), dict(ldy=63), dict(N=(1 << 24) + 1)):
+        assert call(**kw) == _lib.NK_ERR_SHAPE, kw
+    for kw in (dict(codes=at(8)), dict(scales=at(2)), dict(zeros=at(1)), dict(x=at(1)),
+               dict(y=at(1))):
+        assert call(**kw) == _lib.NK_ERR_ALIGN, kw
+
+
+def test_append_q8_abi_refusals():
+    L = _lib.load()
+    p = 1 << 20
+    ok = dict(qkv=p, ld=48 * 128, qn=p, kn=p, cos=p, sin=p, pos=p, per=1, q=p, k=p, v=p, ks=p, vs=p,
+              batch=2, tokens=1, hq=32, hkv=8, d=128, cap=64, block=16, cb=8 * 64 * 128,
+              ch=64 * 128, cs=128, eps=1e-6, stream=None)
+
+    def call(**kw):
+        return L.nk_qk_norm_rope_cache_q8(*(ok | kw).values())
+
+    for n in ("qkv", "qn", "kn", "cos", "sin", "pos", "q", "k", "v", "ks", "vs"):
+        assert call(**{n: None}) == _lib.NK_ERR_ARG, n
+    for kw in (dict(batch=0), dict(batch=1025), dict(tokens=0), dict(tokens=17), dict(hq=0),
+               dict(hkv=0), dict(hq=33), dict(d=64), dict(cap=0), dict(tokens=16, cap=15),
+               dict(block=8), dict(block=48), dict(block=256), dict(ld=48 * 128 - 4), dict(cs=64)):
+        assert call(**kw) == _lib.NK_ERR_SHAPE, kw
+    for kw in (dict(qkv=p + 4), dict(q=p + 2), dict(k=p + 8), dict(v=p + 4), dict(ks=p + 2),
+               dict(pos=p + 4), dict(ld=48 * 128 + 2), dict(cs=136), dict(ch=64 * 128 + 8),
+               dict(cb=8 * 64 * 128 + 4), dict(cos=p + 2)):
+        assert call(**kw) == _lib.NK_ERR_ALIGN, kw
+
+
+def test_attention_q8_abi_refusals():
+    L = _lib.load()
+    p = 1 << 20
+    need = L.nk_attention_q8_ws_bytes(1, 32, 8)
+    assert need > 0
+    ok = dict(q=p, k=p, v=p, ks=p, vs=p, pos=p, per=0, out=p, batch=2, tokens=1, hq=32, hkv=8,
+              d=128, cap=64, block=64, cb=8 * 64 * 128, ch=64 * 128, cs=128, scale=0.1, ws=p,
+              n=need, stream=None)
+
+    def call(**kw):
+        return L.nk_attention_decode_q8(*(ok | kw).values())
+
+    for n in ("q", "k", "v", "ks", "vs", "pos", "out"):
+        assert call(**{n: None}) == _lib.NK_ERR_ARG, n
+    for kw in (dict(batch=0), dict(batch=1025), dict(tokens=0), dict(tokens=17), dict(hkv=0),
+               dict(hq=33), dict(hq=136), dict(d=64), dict(cap=0), dict(tokens=2, cap=1),
+               dict(block=1), dict(cs=112), dict(cap=2 ** 31 - 1, batch=1024)):
+        assert call(**kw) == _lib.NK_ERR_SHAPE, kw
+    for kw in (dict(ws=None), dict(n=need - 1), dict(tokens=16)):
+        assert call(**kw) == _lib.NK_ERR_WORKSPACE, kw
+    for kw in (dict(q=p + 4), dict(out=p + 2), dict(k=p + 8), dict(v=p + 1), dict(ws=p + 8),
+               dict(ks=p + 1), dict(cs=130), dict(ch=4), dict(cb=12), dict(pos=p + 4)):
+        assert call(**kw) == _lib.NK_ERR_ALIGN, kw
+
+
+def test_attention_q8_workspace_sizes():
+    L = _lib.load()
+    assert L.nk_attention_q8_ws_bytes(0, 32, 8) == 0
+    assert L.nk_attention_q8_ws_bytes(17, 32, 8) == 0
+    assert L.nk_attention_q8_ws_bytes(1, 33, 8) == 0
+    assert L.nk_attention_q8_ws_bytes(1, 136, 8) == 0
+    sizes = [L.nk_attention_q8_ws_bytes(t, 64, 8) for t in range(1, 17)]
+    assert sizes == sorted(sizes)  # a workspace for T tokens serves fewer
+
+
+def test_q8_cache_refuses_cpu_tensors_and_bad_blocks():
+    k = torch.zeros(1, 2, 64, 128, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    s = torch.zeros(1, 2, 1)
+    with pytest.raises(ValueError):
+        ops.Q8Cache(k, k.clone(), s, s.clone(), 64)
+    with pytest.raises(ValueError):
+        ops.Q8Cache.empty(1, 2, 64, "cpu", block=24)
+    with pytest.raises(ValueError):
+        ops.Q8Cache.empty(1, 2, 64, "cpu", layout="sbhd")
