@@ -23,16 +23,15 @@ extern "C" {
  * q: 4-bit codes 0..15, s: bf16 or fp16 scales, z: zero points 0..15 (8 when there are none);
  * differences and products exact, sums in fp32, one rounding at the end.
  *
- * Storage, laid out once when the weights are loaded (KB = ceil(K / 128), NB = ceil(N / 16),
- * GP = KB * 128 / group; codes, scales and zero points past K or N are 0):
- *   codes:  [NB][KB][2][32] 16-byte pieces. Piece (i, b, half, lane) holds row
- *           n = 16 i + 8 half + lane / 4; its 32-bit word j (0..3) holds
- *           k = 128 b + 32 j + 8 (lane % 4) + 0..7: element 2 p in bits [4p, 4p + 4) and element
- *           2 p + 1 in bits [16 + 4p, 20 + 4p), p = 0..3. One warp load of a piece row is 512
- *           contiguous bytes, and masking (word >> 4p) with 0x000f000f gives one operand
- *           register of the matrix instruction.
- *   scales: [NB][GP][8][2] 16-bit, element (i, g, r, half) of row 16 i + 8 half + r.
- *   zeros:  [NB][GP][8][2] bytes, same order (NULL: every zero point is 8).
+ * Storage, laid out once when the weights are loaded (KB = ceil(K / 128), NB = ceil(N / 128);
+ * codes, scales and zero points past K or N are 0):
+ *   codes:  [NB][KB][4][128] 16-byte pieces. Piece (i, b, c, r) holds row n = 128 i + r; its 32-bit
+ *           word j (0..3) holds k = 128 b + 32 c + 8 j + 0..7: element 2 p in bits [4p, 4p + 4) and
+ *           element 2 p + 1 in bits [16 + 4p, 20 + 4p), p = 0..3. A step of 128 rows by 128 K is 8 KB
+ *           in one piece, and masking (word >> 4p) with 0x000f000f gives a pair of neighbours in
+ *           the halves of a register.
+ *   scales: [NB][KB][128 / group][128] 16-bit, row 128 i + r last.
+ *   zeros:  the same order, bytes (NULL: every zero point is 8).
  */
 #define NK_W4_SCALE_BF16 0
 #define NK_W4_SCALE_FP16 1
@@ -43,8 +42,8 @@ NK_API size_t nk_w4_code_bytes(int N, int K);
 NK_API size_t nk_w4_scale_bytes(int N, int K, int group);
 NK_API size_t nk_w4_zero_bytes(int N, int K, int group);
 
-/* x: [M, K] bf16, row stride ldx >= K (elements); y: [M, N] bf16, row stride ldy >= N. codes and
- * scales 16-byte aligned, zeros 2-byte aligned or NULL; x and y 2-byte aligned (x 16-byte aligned with
+/* x: [M, K] bf16, row stride ldx >= K (elements); y: [M, N] bf16, row stride ldy >= N. codes,
+ * scales and zeros (or NULL) 16-byte aligned; x and y 2-byte aligned (x 16-byte aligned with
  * ldx % 8 == 0 is read in 16-byte pieces). Any M >= 1. No workspace. The weights must have been
  * written before the launch that precedes this one on the stream (they are read ahead of it);
  * weights made at load time always are. */

@@ -6,74 +6,77 @@
 // cores add exact products in fp32 and the group's scale multiplies that fp32 sum: nothing is
 // rounded before the one rounding of y.
 //
-// What bounds it: at decode batches the weight bytes (half a byte each) over HBM. Per SM that
-// stream brings about 46 weights a clock, so widening them must cost little: a code becomes a
-// bf16 by OR-ing it under the exponent of 128 (0x4300 | q = 128 + q) and subtracting 128 + z, two
-// codes per instruction, in the registers of the lane that loaded them, and goes straight into
-// mma.sync m16n8k16 with the weights as the 16-row operand and eight tokens as its columns (a
-// shared-memory operand would cost four times the weight bytes again in stores). The weights'
-// storage is that operand's register layout, so a warp's loads are whole 512-byte rows.
+// What bounds it: at decode batches the weight bytes (half a byte each) over HBM, some 46 weights
+// a clock and SM, each of which has to be widened. A 16-bit word 0x00vv is the bf16 number vv *
+// 2^-133 (the format's subnormals and first binade are one straight line), so masking a word of
+// codes leaves pairs q * 2^-133 or 16 q * 2^-133, and one fma.bf16x2 with 2^127 or 2^123 and -z
+// 2^-6 makes them (q - z) 2^-6, exactly: nine instructions per eight codes. Shared memory could not
+// take the widened weights (four times the stream again), tensor memory can: the weights are the
+// MMA's A operand there (128 rows = 128 lanes), the tokens its B operand in shared memory.
 //
-// A CTA is eight warps: RW row tiles of 16 weight rows by KW = 8 / RW interleaved K steps (128
-// wide). Activations of the CTA's K range go through shared memory in chunks, in operand order.
-// CTAs of a cluster share a row tile and split K; partials are added in a fixed order, through
-// shared memory within a CTA and distributed shared memory across the cluster, so there is no
-// workspace and no order that changes between runs.
+// A CTA takes 128 weight rows and a range of K steps (128 wide). Its warps:
+//   0      lane 0 streams codes, scales and zero points of each step (one contiguous 8 KB piece
+//          and two small ones) through a ring of bulk copies
+//   1      lane 0 issues the MMAs: 8 per step, the accumulator started anew for each group
+//   2, 3   bring each step's activations into shared memory, 128-byte swizzled
+//   fold   (4 warps, 8 for 64 tokens) take each group's sums out of tensor memory, multiply by the
+//          row's scale and add, in fp32 registers (one thread = one weight row)
+//   widen  (8 warps, 4 for 64 tokens) turn a step's codes into the A operand (one thread = one row)
+// Two CTAs share an SM. Where there are few rows, CTAs of a cluster share them and split K; their
+// fp32 sums are added in rank order through distributed shared memory, after tensor memory is
+// given back (so no CTA that holds some ever waits for another). No workspace, and no order of
+// additions that changes between runs.
+//
+// Every mbarrier wait is bounded: on expiry the thread records NK_ERR_TIMEOUT in the device error
+// word, its role ends, and the CTA drains its copies and MMAs (bounded), stores nothing, frees
+// its tensor memory and exits.
 #include "nk_common.cuh"
 #include "../../include/nk_quant.h"
 
 namespace nk {
 
-constexpr int kW4Threads = 256;
-constexpr int kW4Warps = 8;
+constexpr int kW4Threads = 512;
 constexpr int kW4MaxCluster = 8;
+constexpr int kW4Rows = 128;
+constexpr int kW4StepBytes = kW4Rows * 64;  // codes of one step
 
 struct W4Args {
     const __nv_bfloat16* x; int64_t ldx;
-    const uint4* codes;
-    const uint32_t* scales;       // pairs of rows (r, r + 8)
-    const uint16_t* zeros;        // pairs of rows, or nullptr
+    const uint8_t* codes;
+    const uint8_t* scales;
+    const uint8_t* zeros;
     __nv_bfloat16* y; int64_t ldy;
     int M, N, K;
-    int KB, NB;                   // K steps of 128, row tiles of 16
-    int rw;                       // row tiles per CTA (1, 2, 4 or 8)
-    int chunk;                    // K steps staged together
-    int nbuf;                     // staging buffers (1 when one chunk holds the CTA's range)
-    int fp16_scales;
+    int KB;                       // K steps of 128
     int wide_x;                   // x rows may be read in 16-byte pieces
 };
 
-__device__ __forceinline__ void mma_w4(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                       uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// (word >> 4p) & 0x000f000f under bf16's 128: two codes as bf16 128 + q, minus 128 + z.
-__device__ __forceinline__ uint32_t w4_pair(uint32_t word, int p, __nv_bfloat162 base) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xEA;" : "=r"(r) : "r"(word >> (4 * p)));
-    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&r), base);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-__device__ __forceinline__ float w4_scale(uint32_t bits16, int fp16_scales) {
-    if (fp16_scales) return __half2float(__ushort_as_half((unsigned short)bits16));
-    return __uint_as_float(bits16 << 16);
-}
-
-__device__ __forceinline__ uint32_t ld_nc_u32(const void* p) {
-    uint32_t v;
-    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t ld_nc_u16(const void* p) {
-    uint16_t v;
-    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"(p));
-    return v;
-}
+template <int NT, int NG>
+struct W4Smem {
+    static constexpr int kScale = NG * kW4Rows * 2, kZero = NG * kW4Rows;
+    static constexpr int kW = kW4StepBytes + kScale + kZero;  // one step of weights
+    static constexpr int kX = NT * 256;                       // one step of activations: two boxes
+    static constexpr int kXStages = NT == 16 ? 12 : (NT == 32 ? 6 : 4);
+    static constexpr int kBudget = 112 * 1024;                // two CTAs per SM
+    static constexpr int kFit = (kBudget - 2048 - kXStages * kX) / kW;
+    static constexpr int kWStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kAccs = NT <= 32 ? 4 : 2;            // accumulators in tensor memory
+    static constexpr int kTmemA = 2 * 64;                     // two A buffers of 64 columns
+    static constexpr int kTmemCols = 256;
+    static constexpr int kWOff = kXStages * kX;
+    static constexpr int kBarOff = kWOff + kWStages * kW;
+    static constexpr int kGroupBars = 4;                      // at least kAccs and NG - 1
+    static constexpr int kBars = 2 * kWStages + 2 * kXStages + 2 + kGroupBars + kAccs + 1;
+    static constexpr int kMiscOff = kBarOff + kBars * 8;
+    static constexpr int kAlloc = kMiscOff + 16 + 1024;       // slack to align the base to 1 KB
+    static constexpr int kFoldHalves = NT <= 32 ? 1 : 2;      // fold warps per lane quarter
+    static constexpr int kWidenSets = NT <= 32 ? 2 : 1;       // sets of four widening warps
+    static_assert(kTmemA + kAccs * NT <= kTmemCols, "tensor memory");
+    static_assert(kAccs <= kGroupBars && NG - 1 <= kGroupBars, "group barriers");
+    static_assert(NT * kW4Rows * 4 <= kWOff, "the sums must fit over the activations");
+    static_assert(4 + 4 * kFoldHalves + 4 * kWidenSets == kW4Threads / 32, "roles");
+    static_assert(kW % 128 == 0 && kX % 1024 == 0 && kWStages >= 4, "ring layout");
+};
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -99,6 +102,78 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t saddr, uint32_t rank) {
     return v;
 }
 
+// Bulk copy into this CTA's shared memory, lines marked to leave L2 first (weights are read once).
+__device__ __forceinline__ void bulk_load_hint(uint32_t dst, const void* src, uint32_t bytes,
+                                               uint32_t bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+                 " [%0], [%1], %2, [%3], %4;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)),
+                 "r"(bytes), "r"(bar), "l"(policy) : "memory");
+}
+
+// D[128 rows, N tokens] (+)= A[128 rows, 16] in tensor memory x B in shared memory.
+__device__ __forceinline__ void tc_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
+                                          uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 16 registers per thread -> 32 lanes x 16 consecutive 32-bit columns of tensor memory.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+        " {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15])
+        : "memory");
+}
+
+// Wait for the phase with the given parity, for two seconds at most (then false, error recorded).
+__device__ __forceinline__ bool w4_wait(uint32_t bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    do {
+#pragma unroll 1
+        for (int i = 0; i < 64; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+    } while (global_ns() - t0 < 2000000000ull);
+    atomicExch(&g_error, NK_ERR_TIMEOUT);
+    return false;
+}
+
+__device__ __forceinline__ bool elect_one() {  // true in one lane of the converged warp
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(p));
+    return p != 0;
+}
+
+// Codes at bits 0..3 (HI = 0) or 4..7 (HI = 1) of the word's halves as bf16 pairs
+// (q - z) 2^-6; zc: -z 2^-6 in both halves.
+template <int HI>
+__device__ __forceinline__ uint32_t w4_pair(uint32_t word, uint32_t zc) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;"
+        : "=r"(r)
+        : "r"(word & (HI ? 0x00f000f0u : 0x000f000fu)), "r"(HI ? 0x7d007d00u : 0x7f007f00u), "r"(zc));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t w4_zero(uint32_t z) {  // -z 2^-6 as a bf16 pair
+    return __byte_perm(__float_as_uint((float)z * -0x1p-6f), 0u, 0x3232);
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+    return r;
+}
+
 // 16 bytes of x to shared memory, the first `bytes` of them (0, 2, .. 16) from memory, the rest 0.
 __device__ __forceinline__ void w4_stage16(uint32_t dst, const __nv_bfloat16* src, int bytes,
                                            bool wide) {
@@ -116,265 +191,420 @@ __device__ __forceinline__ void w4_stage16(uint32_t dst, const __nv_bfloat16* sr
     }
 }
 
-// One K step (128 wide) of one 16-row tile in registers: two 16-byte code pieces (rows g and
-// g + 8) and the NG = 128 / group scale and zero-point pairs.
-template <int NG, bool ZP>
-struct W4Step {
-    uint4 w0, w1;
-    uint32_t sc[NG];
-    uint32_t zp[ZP ? NG : 1];
-};
-
-// NT: token tiles of eight; NG: groups per K step; ZP: zero points given; D: K steps in flight per
-// warp.
-template <int NT, int NG, bool ZP, int D>
+// NT: token tile (16, 32 or 64); NG: groups per K step; ZP: zero points given; FP16: scales are
+// fp16, else bf16.
+template <int NT, int NG, bool ZP, bool FP16>
 __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
-    extern __shared__ __align__(128) uint8_t w4_smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int g = lane >> 2, t = lane & 3;
-    const int rw = a.rw, kw = kW4Warps / rw;
-    const int rt = warp % rw, kp = warp / rw;
+    using L = W4Smem<NT, NG>;
+    constexpr int WS = L::kWStages, XS = L::kXStages, DB = L::kAccs;
+    constexpr int FH = L::kFoldHalves, SETS = L::kWidenSets;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t* gbase = smem_raw + (base - raw);
+
+    // (the shuffles tell the compiler that a value is the same in every lane)
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int S = (int)cluster_size(), rank = (int)cluster_rank();
-    const int row_block = blockIdx.x / S;           // the cluster's rows
-    const int tile = row_block * rw + rt;           // 16-row tile of this warp
-    const int m0 = blockIdx.y * (8 * NT);
-    const int mcount = min(8 * NT, a.M - m0);
+    const int tile = blockIdx.x / S;
+    const int m0 = blockIdx.y * NT;
+    const int mcount = min(NT, a.M - m0);
     const int k_begin = (int)((int64_t)rank * a.KB / S);
-    const int k_end = (int)((int64_t)(rank + 1) * a.KB / S);
-    const bool live = tile < a.NB;
+    const int n = (int)((int64_t)(rank + 1) * a.KB / S) - k_begin;  // steps, at least one
 
-    auto load = [&](int st, W4Step<NG, ZP>& r) {
-        if (!live || st >= k_end) return;
-        const uint4* c = a.codes + ((int64_t)tile * a.KB + st) * 64 + lane;
-        r.w0 = ld_stream_v4(c);
-        r.w1 = ld_stream_v4(c + 32);
-        const int64_t s0 = ((int64_t)tile * a.KB + st) * NG * 8 + g;
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            r.sc[i] = ld_nc_u32(a.scales + s0 + i * 8);
-            if (ZP) r.zp[i] = ld_nc_u16(a.zeros + s0 + i * 8);
+    const uint32_t bar_full = base + L::kBarOff;         // weights of a step have landed
+    const uint32_t bar_empty = bar_full + WS * 8;        // ... and are used up
+    const uint32_t bar_xfull = bar_empty + WS * 8;       // activations of a step are there
+    const uint32_t bar_done = bar_xfull + XS * 8;        // a step's MMAs have finished
+    const uint32_t bar_afull = bar_done + XS * 8;        // a step is widened
+    const uint32_t bar_dfull = bar_afull + 2 * 8;        // a group that is not its step's last is summed
+    const uint32_t bar_dempty = bar_dfull + L::kGroupBars * 8;
+    const uint32_t bar_drain = bar_dempty + DB * 8;
+    volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(gbase + L::kMiscOff);
+    volatile uint32_t* abort_flag = misc + 1;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < WS; ++i) {
+            mbar_init(bar_full + 8 * i, 1);
+            mbar_init(bar_empty + 8 * i, 4 + 4 * FH);
         }
-    };
-
-    W4Step<NG, ZP> q[D];
-    // the weights do not depend on the previous launch: their first loads go out before the wait
-#pragma unroll
-    for (int d = 0; d < D; ++d) load(k_begin + kp + d * kw, q[d]);
+        for (int i = 0; i < XS; ++i) {
+            mbar_init(bar_xfull + 8 * i, 2);
+            mbar_init(bar_done + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) mbar_init(bar_afull + 8 * i, 4);
+        for (int i = 0; i < L::kGroupBars; ++i) mbar_init(bar_dfull + 8 * i, 1);
+        for (int i = 0; i < DB; ++i) mbar_init(bar_dempty + 8 * i, 4 * FH);
+        mbar_init(bar_drain, 1);
+        *abort_flag = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32((const void*)misc)),
+                     "r"((uint32_t)L::kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, misc[0], 0);
     if (threadIdx.x == 0) griddep_launch_dependents();
-    griddep_wait();
 
-    const uint32_t s0 = static_cast<uint32_t>(__cvta_generic_to_shared(w4_smem));
-    const int buf_bytes = a.chunk * NT * 2048;
-    auto stage = [&](int c0, int buf) {  // K steps [c0, c0 + chunk) of every token
-        const int steps = min(a.chunk, k_end - c0);
-        const int pieces = steps * 16;
-        const uint32_t base = s0 + buf * buf_bytes;
-        for (int i = threadIdx.x; i < pieces * 8 * NT; i += kW4Threads) {
-            const int m = i / pieces, c = i - m * pieces;  // token, 8-wide piece of the chunk
-            const int k = c0 * 128 + c * 8;
-            const int n = m < mcount ? min(max(a.K - k, 0), 8) : 0;
-            const uint32_t dst = base + ((c >> 2) * NT + (m >> 3)) * 512 + ((m & 7) * 4 + (c & 3)) * 16;
-            const __nv_bfloat16* src = n > 0 ? a.x + (int64_t)(m0 + m) * a.ldx + k : a.x;
-            w4_stage16(dst, src, 2 * n, a.wide_x != 0);
+    constexpr int kFold0 = 4, kWiden0 = 4 + 4 * FH;
+    // A group's barrier completes once per round of the index that names it, and no second time
+    // before the fold warps have seen the first: by accumulator where a round of the DB
+    // accumulators holds two steps' groups, else by the group's place in its step (the MMAs are
+    // never a whole step of groups ahead of the fold warps there).
+    constexpr bool kByAcc = DB == 4 && NG == 2;
+    static_assert(kByAcc || DB <= NG || NG == 1, "group barriers");
+    // The done barrier of a step comes round after XS steps; fold warps lag by at most DB groups.
+    static_assert(XS >= DB && XS >= 3, "done barriers");
+    if (warp == 0) {
+        if (lane == 0) {
+            // weights do not depend on the previous launch: no wait for it
+            const uint64_t policy = l2_evict_first_policy();
+            const int64_t at = (int64_t)tile * a.KB + k_begin;
+            const uint8_t* codes = a.codes + at * kW4StepBytes;
+            const uint8_t* scales = a.scales + at * L::kScale;
+            const uint8_t* zeros = ZP ? a.zeros + at * L::kZero : nullptr;
+            int i = 0;
+            for (; i < n; ++i) {
+                const int st = i % WS;
+                if (i >= WS && !w4_wait(bar_empty + 8 * st, (i / WS - 1) & 1)) {
+                    *abort_flag = 1u;
+                    break;
+                }
+                const uint32_t dst = base + L::kWOff + st * L::kW, bar = bar_full + 8 * st;
+                mbar_expect_tx(bar, kW4StepBytes + L::kScale + (ZP ? L::kZero : 0));
+                bulk_load_hint(dst, codes + (int64_t)i * kW4StepBytes, kW4StepBytes, bar, policy);
+                bulk_load_hint(dst + kW4StepBytes, scales + (int64_t)i * L::kScale, L::kScale, bar,
+                               policy);
+                if (ZP)
+                    bulk_load_hint(dst + kW4StepBytes + L::kScale, zeros + (int64_t)i * L::kZero,
+                                   L::kZero, bar, policy);
+            }
+            if (i < n)  // stopped: the copies in flight must land before the CTA goes
+                for (int j = i > WS ? i - WS : 0; j < i; ++j)
+                    w4_wait(bar_full + 8 * (j % WS), (j / WS) & 1);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-
-    float acc[NT][4];
+    } else if (warp == 1) {
+        // the whole warp walks the loop, so that descriptors stay in uniform registers
+        constexpr uint32_t idesc = tc_idesc(kW4Rows, NT);
+        const bool leader = elect_one();
+        bool ok = true;
+        int xs = 0, xph = 0, db = 0, dph = 1;
+#pragma unroll 1
+        for (int i = 0; i < n && ok; ++i) {
+            const uint32_t ab = i & 1;
+            ok = w4_wait(bar_xfull + 8 * xs, xph) && w4_wait(bar_afull + 8 * ab, (i >> 1) & 1);
+            if (!ok) break;
+            const uint64_t bdesc = sw128_desc(base + xs * L::kX);
+            const uint32_t ta = tmem + ab * 64;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-
-    auto compute = [&](const W4Step<NG, ZP>& r, uint32_t xs) {  // xs: the step's operand pieces
-        constexpr int WPG = 4 / NG;  // words per group
-        const uint32_t w0[4] = {r.w0.x, r.w0.y, r.w0.z, r.w0.w};
-        const uint32_t w1[4] = {r.w1.x, r.w1.y, r.w1.z, r.w1.w};
+            for (int j = 0; j < NG; ++j) {
+                ok = w4_wait(bar_dempty + 8 * db, dph);  // passes at once for the first DB groups
+                if (!ok) break;
+                tc_fence_after();
+                if (leader) {
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            __nv_bfloat162 z0, z1;
-            if (ZP) {
-                z0 = __bfloat162bfloat162(__ushort_as_bfloat16(0x4300u | (r.zp[i] & 0xffu)));
-                z1 = __bfloat162bfloat162(__ushort_as_bfloat16(0x4300u | (r.zp[i] >> 8)));
+                    for (int k = 0; k < 8 / NG; ++k) {
+                        const int kk = j * (8 / NG) + k;
+                        tc_mma_ts(tmem + L::kTmemA + db * NT, ta + kk * 8,
+                                  bdesc + (((kk >> 2) * (NT * 128) + 32 * (kk & 3)) >> 4), idesc,
+                                  k > 0);
+                    }
+                    tc_commit(j == NG - 1 ? bar_done + 8 * xs : bar_dfull + 8 * (kByAcc ? db : j));
+                }
+                __syncwarp();
+                if (++db == DB) {
+                    db = 0;
+                    dph ^= 1;
+                }
+            }
+            if (++xs == XS) {
+                xs = 0;
+                xph ^= 1;
+            }
+        }
+        if (!ok) {
+            *abort_flag = 1u;
+            if (leader) tc_commit(bar_drain);
+            __syncwarp();
+            w4_wait(bar_drain, 0);
+        }
+    } else if (warp < kFold0) {
+        // 64 threads: piece c (8 wide) of tokens r, r + 4, ..; LEAD steps ahead of the MMAs
+        constexpr int LEAD = XS - 2;
+        griddep_wait();  // x is the previous launch's
+        const int tid = threadIdx.x - 64, c = tid & 15, r = tid >> 4;
+        const __nv_bfloat16* src = a.x + (int64_t)(m0 + r) * a.ldx + k_begin * 128 + c * 8;
+        const uint32_t dst = base + (c >> 3) * (NT * 128) + r * 128;
+        const uint32_t sw0 = ((c & 7) ^ r) << 4, sw1 = ((c & 7) ^ (r + 4)) << 4;
+        const int64_t row4 = 4 * a.ldx;
+        const bool wide = a.wide_x != 0;
+        const int left = a.K - k_begin * 128 - c * 8;  // elements from the first step's piece on
+        auto issue = [&](int i, int xs) {
+            const int bytes = 2 * min(max(left - i * 128, 0), 8);
+            const __nv_bfloat16* p = bytes > 0 ? src + i * 128 : a.x;
+            const int64_t next = bytes > 0 ? row4 : 0;
+            uint32_t d = dst + xs * L::kX;
+            // columns of tokens past mcount stay as they are: they only reach sums never stored
+#pragma unroll 1
+            for (int m = r; m < mcount; m += 4, p += next, d += 512)
+                w4_stage16(d + ((m & 4) ? sw1 : sw0), p, bytes, wide);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        bool ok = true;
+        for (int i = 0; i < min(n, LEAD); ++i) issue(i, i);
+        for (int i = n; i < LEAD; ++i) asm volatile("cp.async.commit_group;" ::: "memory");
+        int xs = 0, ahead = LEAD, aph = 1;  // aph: parity of step i + LEAD's predecessor in its slot
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(LEAD - 1) : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_xfull + 8 * xs);
+            if (++xs == XS) xs = 0;
+            if (i + LEAD < n) {
+                ok = w4_wait(bar_done + 8 * ahead, aph);  // passes at once for the first XS steps
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                issue(i + LEAD, ahead);
             } else {
-                z0 = z1 = __bfloat162bfloat162(__ushort_as_bfloat16(0x4308u));
+                asm volatile("cp.async.commit_group;" ::: "memory");
             }
-            float part[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.f;
-#pragma unroll
-            for (int jj = 0; jj < WPG; ++jj) {
-                const int j = i * WPG + jj;
-                uint32_t f0[4], f1[4];
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    f0[p] = w4_pair(w0[j], p, z0);
-                    f1[p] = w4_pair(w1[j], p, z1);
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    uint32_t b0, b1, b2, b3;
-                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                                 : "=r"(b0), "=r"(b1), "=r"(b2), "=r"(b3)
-                                 : "r"(xs + (j * NT + n) * 512 + lane * 16));
-                    mma_w4(part[n], f0[0], f1[0], f0[1], f1[1], b0, b1);
-                    mma_w4(part[n], f0[2], f1[2], f0[3], f1[3], b2, b3);
-                }
-            }
-            const float sa = w4_scale(r.sc[i] & 0xffffu, a.fp16_scales);
-            const float sb = w4_scale(r.sc[i] >> 16, a.fp16_scales);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                acc[n][0] = fmaf(sa, part[n][0], acc[n][0]);
-                acc[n][1] = fmaf(sa, part[n][1], acc[n][1]);
-                acc[n][2] = fmaf(sb, part[n][2], acc[n][2]);
-                acc[n][3] = fmaf(sb, part[n][3], acc[n][3]);
+            if (++ahead == XS) {
+                ahead = 0;
+                aph ^= 1;
             }
         }
-    };
-
-    // chunk = kw * D * m steps, so every warp takes D * m steps of a whole chunk and slot d of its
-    // queue is always step kp + (..D + d) * kw of it
-    stage(k_begin, 0);
-    int buf = 0;
-    for (int c0 = k_begin; c0 < k_end; c0 += a.chunk) {
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncthreads();  // the chunk is staged; everyone is done with the other buffer
-        if (c0 + a.chunk < k_end) stage(c0 + a.chunk, buf ^ 1);
-        const int c1 = min(c0 + a.chunk, k_end);
-        const uint32_t xb = s0 + buf * buf_bytes;
-        for (int st = c0 + kp; st < c1; st += kw * D) {
+        if (!ok) *abort_flag = 1u;
+    } else if (warp < kWiden0) {
+        const int quarter = warp & 3, half = (warp - kFold0) >> 2;
+        const int row = quarter * 32 + lane;
+        constexpr int COLS = NT / FH;
+        const uint32_t taddr = tmem + L::kTmemA + ((uint32_t)(quarter * 32) << 16) + half * COLS;
+        float acc[COLS];
 #pragma unroll
-            for (int d = 0; d < D; ++d) {
-                const int s = st + d * kw;
-                if (s < c1) {
-                    if (live) compute(q[d], xb + (s - c0) * (NT * 2048));
-                    load(s + kw * D, q[d]);
+        for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
+        bool ok = true;
+        int st = 0, wph = 0, xs = 0, xph = 0, db = 0, dph = 0;
+#pragma unroll 1
+        for (int i = 0; i < n && ok; ++i) {
+            ok = __all_sync(0xffffffffu, w4_wait(bar_full + 8 * st, wph));
+            if (!ok) break;
+            const uint8_t* sc = gbase + L::kWOff + st * L::kW + kW4StepBytes + row * 2;
+            float s[NG];
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                const uint16_t bits = *reinterpret_cast<const uint16_t*>(sc + j * kW4Rows * 2);
+                s[j] = FP16 ? __half2float(__ushort_as_half(bits))
+                            : __uint_as_float((uint32_t)bits << 16);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_empty + 8 * st);
+            if (++st == WS) {
+                st = 0;
+                wph ^= 1;
+            }
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                ok = __all_sync(0xffffffffu,
+                                j == NG - 1 ? w4_wait(bar_done + 8 * xs, xph)
+                                            : w4_wait(bar_dfull + 8 * (kByAcc ? db : j),
+                                                        kByAcc ? dph : i & 1));
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < COLS; c += 16) {
+                    float v[16];
+                    tmem_ld16(taddr + db * NT + c, v);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(s[j], v[e], acc[c + e]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_dempty + 8 * db);
+                if (++db == DB) {
+                    db = 0;
+                    dph ^= 1;
                 }
             }
+            if (++xs == XS) {
+                xs = 0;
+                xph ^= 1;
+            }
         }
-        buf ^= 1;
+        if (!ok) *abort_flag = 1u;
+        // Every MMA has finished (the last group's sums are read), so the activations' ring may hold
+        // the sums: [token][row], out of the codes' unit 2^-6.
+        if (ok) {
+            float* red = reinterpret_cast<float*>(gbase) + half * COLS * kW4Rows + row;
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) red[c * kW4Rows] = acc[c] * 64.f;
+        }
+    } else {
+        const int quarter = warp & 3, set = (warp - kWiden0) >> 2;
+        const int row = quarter * 32 + lane;
+        bool ok = true;
+        int st = set, wph = 0, xs = XS - 2 + set, xph = 1;  // xs, xph: of step i - 2
+#pragma unroll 1
+        for (int i = set; i < n; i += SETS) {
+            const uint32_t ab = i & 1;
+            ok = __all_sync(0xffffffffu, w4_wait(bar_full + 8 * st, wph));
+            if (!ok) break;
+            const uint32_t w = base + L::kWOff + st * L::kW;
+            uint32_t zc[NG];
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+                zc[j] = ZP ? w4_zero(gbase[L::kWOff + st * L::kW + kW4StepBytes + L::kScale +
+                                           j * kW4Rows + row])
+                           : 0xbe00be00u;
+            uint4 u[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) u[c] = lds128(w + c * 2048 + row * 16);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_empty + 8 * st);
+            // the MMAs of step i - 2 have read this buffer (passes at once for the first two)
+            ok = __all_sync(0xffffffffu, w4_wait(bar_done + 8 * xs, xph));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16) + ab * 64;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {  // 32 K elements: one group or part of one
+                const uint32_t z = zc[c * NG / 4];
+                const uint32_t word[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+                uint32_t r[16];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    r[4 * k] = w4_pair<0>(word[k], z);
+                    r[4 * k + 1] = w4_pair<1>(word[k], z);
+                    r[4 * k + 2] = w4_pair<0>(word[k] >> 8, z);
+                    r[4 * k + 3] = w4_pair<1>(word[k] >> 8, z);
+                }
+                tmem_st16(ta + c * 16, r);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_afull + 8 * ab);
+            if ((st += SETS) >= WS) {
+                st -= WS;
+                wph ^= 1;
+            }
+            if ((xs += SETS) >= XS) {
+                xs -= XS;
+                xph ^= 1;
+            }
+        }
+        if (!ok) *abort_flag = 1u;
     }
 
-    // partial tiles [kp][token][row] in shared memory, over the staging buffers
+    __syncwarp();
+    tc_fence_before();
     __syncthreads();
-    float* red = reinterpret_cast<float*>(w4_smem);
-    const int rows = 16 * rw, elems = rows * 8 * NT;
-    {
-        float* p = red + kp * elems + rt * 16;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            p[(8 * n + 2 * t) * rows + g] = acc[n][0];
-            p[(8 * n + 2 * t + 1) * rows + g] = acc[n][1];
-            p[(8 * n + 2 * t) * rows + g + 8] = acc[n][2];
-            p[(8 * n + 2 * t + 1) * rows + g + 8] = acc[n][3];
-        }
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                     "r"((uint32_t)L::kTmemCols)
+                     : "memory");
     }
-    __syncthreads();
-    const int n0 = row_block * rows;
-    const int count = rows * mcount;
+    griddep_wait();  // outputs may still be read by the previous launch
+    const bool good = *abort_flag == 0u;
+    const float* red = reinterpret_cast<const float*>(gbase);
+    const int count = mcount * kW4Rows, n0 = tile * kW4Rows;
     if (S == 1) {
         for (int e = threadIdx.x; e < count; e += kW4Threads) {
-            float v = red[e];
-            for (int p = 1; p < kw; ++p) v += red[p * elems + e];
-            const int m = e / rows, r = e - m * rows;
-            if (n0 + r < a.N) a.y[(int64_t)(m0 + m) * a.ldy + n0 + r] = __float2bfloat16_rn(v);
+            const int m = e / kW4Rows, r = e % kW4Rows;
+            if (good && n0 + r < a.N)
+                a.y[(int64_t)(m0 + m) * a.ldy + n0 + r] = __float2bfloat16_rn(red[e]);
         }
         return;
     }
-    if (kw > 1) {  // this CTA's sum into slice 0
-        for (int e = threadIdx.x; e < count; e += kW4Threads) {
-            float v = red[e];
-            for (int p = 1; p < kw; ++p) v += red[p * elems + e];
-            red[e] = v;
-        }
-    }
+    // each CTA of the cluster adds its share of the elements, in rank order
     cluster_arrive();
     cluster_wait();
     const int per = (count + S - 1) / S;
-    const uint32_t r0 = s0;
     for (int e = rank * per + threadIdx.x; e < min(count, (rank + 1) * per); e += kW4Threads) {
         float part[kW4MaxCluster];
 #pragma unroll
         for (int s = 0; s < kW4MaxCluster; ++s)
-            if (s < S) part[s] = ld_cluster_f32(r0 + 4 * e, s);
+            if (s < S) part[s] = ld_cluster_f32(base + 4 * e, s);
         float v = part[0];
 #pragma unroll
         for (int s = 1; s < kW4MaxCluster; ++s)
             if (s < S) v += part[s];
-        const int m = e / rows, r = e - m * rows;
-        if (n0 + r < a.N) a.y[(int64_t)(m0 + m) * a.ldy + n0 + r] = __float2bfloat16_rn(v);
+        const int m = e / kW4Rows, r = e % kW4Rows;
+        if (good && n0 + r < a.N)
+            a.y[(int64_t)(m0 + m) * a.ldy + n0 + r] = __float2bfloat16_rn(v);
     }
     cluster_arrive();  // no CTA leaves while another may still read its shared memory
     cluster_wait();
 }
 
-struct W4Plan {
-    int nt, rw, S, chunk, nbuf, smem;
-};
+#ifdef W4_TUNE
+extern "C" { __attribute__((visibility("default"))) int w4_tune_s = 0; }
+#endif
 
-template <int NT, int D>
-static W4Plan w4_plan(int M, int NB, int KB) {
-    W4Plan p;
-    p.nt = NT;
-    p.rw = NT == 1 ? 2 : (NT == 2 ? 4 : 8);
-    const int kw = kW4Warps / p.rw;
-    const int tiles = ((NB + p.rw - 1) / p.rw) * ((M + 8 * NT - 1) / (8 * NT));
-    p.S = 1;
-    while (p.S < kW4MaxCluster && tiles * p.S < 2 * kNumSMs && KB >= 2 * p.S * kw) p.S *= 2;
-    const int range = (KB + p.S - 1) / p.S;  // most K steps of one CTA
-    const int unit = kw * D;
-    int m = (32 * 1024) / (unit * NT * 2048);
-    if (m < 1) m = 1;
-    if (m > (range + unit - 1) / unit) m = (range + unit - 1) / unit;
-    p.chunk = unit * m;
-    p.nbuf = range > p.chunk ? 2 : 1;
-    const int stage = p.nbuf * p.chunk * NT * 2048;
-    const int red = kW4Warps * 16 * 8 * NT * 4;
-    p.smem = stage > red ? stage : red;
-    return p;
-}
-
-template <int NT, int NG, bool ZP, int D>
-static int w4_launch(const W4Args& base, cudaStream_t s) {
-    const W4Plan p = w4_plan<NT, D>(base.M, base.NB, base.KB);
-    W4Args a = base;
-    a.rw = p.rw;
-    a.chunk = p.chunk;
-    a.nbuf = p.nbuf;
-    auto kernel = w4_kernel<NT, NG, ZP, D>;
-    static bool ready[64] = {};  // shared-memory limit raised, per device
+template <int NT, int NG, bool ZP, bool FP16>
+static int w4_launch(const W4Args& a, cudaStream_t s) {
+    using L = W4Smem<NT, NG>;
+    auto kernel = w4_kernel<NT, NG, ZP, FP16>;
+    static int sms[64] = {};  // multiprocessors, once the kernel's shared-memory limit is raised
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return NK_ERR_CUDA;
     if (dev < 0 || dev >= 64) return NK_ERR_DEVICE;
-    if (!ready[dev]) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024) !=
-            cudaSuccess)
+    if (sms[dev] == 0) {
+        int n = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc) !=
+                cudaSuccess ||
+            cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 (int)cudaSharedmemCarveoutMaxShared) != cudaSuccess ||
+            cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
             return NK_ERR_CUDA;
-        ready[dev] = true;
+        sms[dev] = n;
     }
+    const int tiles = (a.N + kW4Rows - 1) / kW4Rows, mt = (a.M + NT - 1) / NT;
+    // K is split while the CTAs still fit the GPU at once and keep two steps each
+    int S = (int)min((int64_t)kW4MaxCluster, (int64_t)2 * sms[dev] / ((int64_t)tiles * mt));
+    S = max(1, min(S, a.KB / 2));
+#ifdef W4_TUNE
+    if (w4_tune_s) S = min(w4_tune_s, a.KB);
+#endif
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.S * ((a.NB + p.rw - 1) / p.rw), (a.M + 8 * NT - 1) / (8 * NT));
+    cfg.gridDim = dim3(tiles * S, mt);
     cfg.blockDim = dim3(kW4Threads);
-    cfg.dynamicSmemBytes = p.smem;
+    cfg.dynamicSmemBytes = L::kAlloc;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = p.S;
+    attr[1].val.clusterDim.x = S;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = S > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? NK_OK : NK_ERR_CUDA;
 }
 
-template <int NT, int D>
-static int w4_dispatch(const W4Args& a, int group, cudaStream_t s) {
-    const bool zp = a.zeros != nullptr;
+template <int NT, int NG>
+static int w4_types(const W4Args& a, bool fp16, cudaStream_t s) {
+    if (a.zeros)
+        return fp16 ? w4_launch<NT, NG, true, true>(a, s) : w4_launch<NT, NG, true, false>(a, s);
+    return fp16 ? w4_launch<NT, NG, false, true>(a, s) : w4_launch<NT, NG, false, false>(a, s);
+}
+
+template <int NT>
+static int w4_dispatch(const W4Args& a, int group, bool fp16, cudaStream_t s) {
     switch (group) {
-        case 32: return zp ? w4_launch<NT, 4, true, D>(a, s) : w4_launch<NT, 4, false, D>(a, s);
-        case 64: return zp ? w4_launch<NT, 2, true, D>(a, s) : w4_launch<NT, 2, false, D>(a, s);
-        default: return zp ? w4_launch<NT, 1, true, D>(a, s) : w4_launch<NT, 1, false, D>(a, s);
+        case 32: return w4_types<NT, 4>(a, fp16, s);
+        case 64: return w4_types<NT, 2>(a, fp16, s);
+        default: return w4_types<NT, 1>(a, fp16, s);
     }
 }
 
@@ -387,12 +617,12 @@ static bool w4_group_ok(int group) { return group == 32 || group == 64 || group 
 
 extern "C" size_t nk_w4_code_bytes(int N, int K) {
     if (!nk::w4_shape_ok(N, K)) return 0;
-    return (size_t)((N + 15) / 16) * (size_t)((K + 127) / 128) * 1024;
+    return (size_t)((N + 127) / 128) * (size_t)((K + 127) / 128) * nk::kW4StepBytes;
 }
 
 extern "C" size_t nk_w4_scale_bytes(int N, int K, int group) {
     if (!nk::w4_shape_ok(N, K) || !nk::w4_group_ok(group)) return 0;
-    return (size_t)((N + 15) / 16) * (size_t)((K + 127) / 128) * (128 / group) * 32;
+    return (size_t)((N + 127) / 128) * (size_t)((K + 127) / 128) * (128 / group) * 256;
 }
 
 extern "C" size_t nk_w4_zero_bytes(int N, int K, int group) {
@@ -407,27 +637,25 @@ extern "C" int nk_gemm_w4(const void* x, int64_t ldx, const void* codes, const v
     if (scale_type != NK_W4_SCALE_BF16 && scale_type != NK_W4_SCALE_FP16) return NK_ERR_ARG;
     if (!w4_shape_ok(N, K) || !w4_group_ok(group) || M < 1 || M > (1 << 20) || ldx < K || ldy < N)
         return NK_ERR_SHAPE;
-    if (((uintptr_t)codes & 15u) || ((uintptr_t)scales & 15u) || ((uintptr_t)zeros & 1u) ||
-        ((uintptr_t)x & 1u) || ((uintptr_t)y & 1u))
+    if ((((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)zeros) & 15u) ||
+        (((uintptr_t)x | (uintptr_t)y) & 1u))
         return NK_ERR_ALIGN;
     W4Args a{};
     a.x = static_cast<const __nv_bfloat16*>(x);
     a.ldx = ldx;
-    a.codes = static_cast<const uint4*>(codes);
-    a.scales = static_cast<const uint32_t*>(scales);
-    a.zeros = static_cast<const uint16_t*>(zeros);
+    a.codes = static_cast<const uint8_t*>(codes);
+    a.scales = static_cast<const uint8_t*>(scales);
+    a.zeros = static_cast<const uint8_t*>(zeros);
     a.y = static_cast<__nv_bfloat16*>(y);
     a.ldy = ldy;
     a.M = M;
     a.N = N;
     a.K = K;
     a.KB = (K + 127) / 128;
-    a.NB = (N + 15) / 16;
-    a.fp16_scales = scale_type == NK_W4_SCALE_FP16;
     a.wide_x = ((uintptr_t)x & 15u) == 0 && ldx % 8 == 0;
+    const bool fp16 = scale_type == NK_W4_SCALE_FP16;
     cudaStream_t s = (cudaStream_t)stream;
-    if (M <= 8) return w4_dispatch<1, 4>(a, group, s);
-    if (M <= 16) return w4_dispatch<2, 4>(a, group, s);
-    if (M <= 32) return w4_dispatch<4, 2>(a, group, s);
-    return w4_dispatch<8, 2>(a, group, s);
+    if (M <= 16) return w4_dispatch<16>(a, group, fp16, s);
+    if (M <= 32) return w4_dispatch<32>(a, group, fp16, s);
+    return w4_dispatch<64>(a, group, fp16, s);
 }

@@ -71,19 +71,19 @@ class W4Weight:
                   and zeros.device == q.device,
                   f"W4Weight: zeros must be uint8 [{N}, {G}] on q's device")
             _need(int(zeros.max()) <= 15, "W4Weight: zero points must be 0..15")
-        NB, KB = -(-N // 16), -(-K // 128)
-        codes = torch.zeros(NB * 16, KB * 128, dtype=torch.uint8, device=q.device)
-        codes[:N, 0:K:2] = (q & 15)[:, :-(-K // 2)]
+        NB, KB = -(-N // 128), -(-K // 128)
+        codes = torch.zeros(NB * 128, KB * 128, dtype=torch.uint8, device=q.device)
+        codes[:N, 0:K:2] = q & 15
         codes[:N, 1:K:2] = (q >> 4)[:, :K // 2]
-        # [tile, half, row, step, word, lane quarter, element] -> [tile, step, half, row, quarter, word]
-        c = codes.view(NB, 2, 8, KB, 4, 4, 8).permute(0, 3, 1, 2, 5, 4, 6)
+        # [tile, row, step, piece, word, element] -> [tile, step, piece, row, word], by byte
+        c = codes.view(NB, 128, KB, 4, 4, 8).permute(0, 2, 3, 1, 4, 5)
         codes = torch.stack([c[..., a] | (c[..., b] << 4) for a, b in ((0, 2), (4, 6), (1, 3), (5, 7))],
                             dim=-1).contiguous().view(-1)
 
-        def rows(t):  # [N, G] -> [tile, group, row, half]
-            p = torch.zeros(NB * 16, KB * 128 // group, dtype=t.dtype, device=t.device)
+        def rows(t):  # [N, G] -> [tile, group, row]
+            p = torch.zeros(NB * 128, KB * 128 // group, dtype=t.dtype, device=t.device)
             p[:N, :G] = t
-            return p.view(NB, 2, 8, -1).permute(0, 3, 2, 1).contiguous().view(-1)
+            return p.view(NB, 128, -1).transpose(1, 2).contiguous().view(-1)
 
         w = cls(N, K, group, codes, rows(scales), rows(zeros) if zeros is not None else None,
                 _SCALE_TYPES[scales.dtype])
@@ -122,15 +122,15 @@ class W4Weight:
 
     def dequantize(self):
         """The weight it stands for, fp32 [N, K]."""
-        NB, KB = -(-self.N // 16), -(-self.K // 128)
-        b = self.codes.view(NB, KB, 2, 8, 4, 4, 4)  # tile, step, half, row, quarter, word, byte
+        NB, KB = -(-self.N // 128), -(-self.K // 128)
+        b = self.codes.view(NB, KB, 4, 128, 4, 4)  # tile, step, piece, row, word, byte
         lo, hi = b & 15, b >> 4
         e = torch.stack((lo[..., 0], lo[..., 2], hi[..., 0], hi[..., 2],
                          lo[..., 1], lo[..., 3], hi[..., 1], hi[..., 3]), dim=-1)
-        q = e.permute(0, 2, 3, 1, 5, 4, 6).reshape(NB * 16, KB * 128).float()
+        q = e.permute(0, 3, 1, 2, 4, 5).reshape(NB * 128, KB * 128).float()
 
         def rows(t):
-            t = t.view(NB, -1, 8, 2).permute(0, 3, 2, 1).reshape(NB * 16, -1).float()
+            t = t.view(NB, -1, 128).transpose(1, 2).reshape(NB * 128, -1).float()
             return t.repeat_interleave(self.group, dim=1)
 
         z = rows(self.zeros) if self.zeros is not None else 8.0

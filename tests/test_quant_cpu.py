@@ -30,24 +30,24 @@ def test_storage_layout(N, K, group, zeros):
     assert w.scales.nbytes == L.nk_w4_scale_bytes(N, K, group)
     if zeros:
         assert w.zeros.nbytes == L.nk_w4_zero_bytes(N, K, group)
-    NB, KB, GP = -(-N // 16), -(-K // 128), -(-K // 128) * 128 // group
-    words = w.codes.view(torch.int32).view(NB, KB, 2, 32, 4)
-    scales, zp = w.scales.view(NB, GP, 8, 2), w.zeros.view(NB, GP, 8, 2) if zeros else None
-    for n in range(NB * 16):
-        i, half, r = n // 16, n % 16 // 8, n % 8
+    NB, KB, GP = -(-N // 128), -(-K // 128), -(-K // 128) * 128 // group
+    words = w.codes.view(torch.int32).view(NB, KB, 4, 128, 4)
+    scales, zp = w.scales.view(NB, GP, 128), w.zeros.view(NB, GP, 128) if zeros else None
+    for n in range(NB * 128):
+        i, r = n // 128, n % 128
         for k in range(0, KB * 128, 7):
-            b, j, quarter, e = k // 128, k % 128 // 32, k % 32 // 8, k % 8
-            word = int(words[i, b, half, 4 * r + quarter, j]) & 0xffffffff
+            b, piece, j, e = k // 128, k % 128 // 32, k % 32 // 8, k % 8
+            word = int(words[i, b, piece, r, j]) & 0xffffffff
             code = word >> (4 * (e // 2) + 16 * (e % 2)) & 15
             if n < N and k < K:
                 assert code == int(q[n, k // 2]) >> 4 * (k % 2) & 15
-                assert scales[i, k // group, r, half] == s[n, k // group]
+                assert scales[i, k // group, r] == s[n, k // group]
                 if zeros:
-                    assert zp[i, k // group, r, half] == z[n, k // group]
+                    assert zp[i, k // group, r] == z[n, k // group]
             else:
                 assert code == 0
                 if n >= N or k // group >= s.shape[1]:
-                    assert scales[i, k // group, r, half] == 0
+                    assert scales[i, k // group, r] == 0
 
 
 @pytest.mark.parametrize("zeros", (False, True))
@@ -110,7 +110,7 @@ def test_gemm_w4_abi_refusals():
     for kw in (dict(M=0), dict(M=-1), dict(M=(1 << 20) + 1), dict(N=0), dict(K=0), dict(group=16),
                dict(group=0), dict(ldx=255), dict(ldy=63), dict(N=(1 << 24) + 1)):
         assert call(**kw) == _lib.NK_ERR_SHAPE, kw
-    for kw in (dict(codes=at(8)), dict(scales=at(2)), dict(zeros=at(1)), dict(x=at(1)),
+    for kw in (dict(codes=at(8)), dict(scales=at(2)), dict(zeros=at(4)), dict(x=at(1)),
                dict(y=at(1))):
         assert call(**kw) == _lib.NK_ERR_ALIGN, kw
 
