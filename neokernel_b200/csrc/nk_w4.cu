@@ -18,7 +18,8 @@
 //   0      lane 0 streams codes, scales and zero points of each step (one contiguous 8 KB piece
 //          and two small ones) through a ring of bulk copies
 //   1      lane 0 issues the MMAs: 8 per step, the accumulator started anew for each group
-//   2, 3   bring each step's activations into shared memory, 128-byte swizzled
+//   2      lane 0 brings each step's activations into shared memory (TMA, 128-byte swizzled); rows
+//          that TMA cannot take are copied by warps 2 and 3
 //   fold   (4 warps, 8 for 64 tokens) take each group's sums out of tensor memory, multiply by the
 //          row's scale and add, in fp32 registers (one thread = one weight row)
 //   widen  (8 warps, 4 for 64 tokens) turn a step's codes into the A operand (one thread = one row)
@@ -48,7 +49,7 @@ struct W4Args {
     __nv_bfloat16* y; int64_t ldy;
     int M, N, K;
     int KB;                       // K steps of 128
-    int wide_x;                   // x rows may be read in 16-byte pieces
+    int wide_x;                   // x rows are 16-byte aligned: TMA reads them
 };
 
 template <int NT, int NG>
@@ -60,13 +61,17 @@ struct W4Smem {
     static constexpr int kBudget = 112 * 1024;                // two CTAs per SM
     static constexpr int kFit = (kBudget - 2048 - kXStages * kX) / kW;
     static constexpr int kWStages = kFit > 8 ? 8 : kFit;
-    static constexpr int kAccs = NT <= 32 ? 4 : 2;            // accumulators in tensor memory
+    static constexpr int kAccs = NT == 16 ? 8 : (NT == 32 ? 4 : 2);  // accumulators in tensor memory
     static constexpr int kTmemA = 2 * 64;                     // two A buffers of 64 columns
     static constexpr int kTmemCols = 256;
+    // Where the accumulators hold two steps' groups, the fold warps' release of a step is one of
+    // the arrivals that a later step's MMAs wait for; else the MMAs wait for each accumulator.
+    static constexpr bool kStepRelease = kAccs >= 2 * NG;
+    static constexpr int kLag = kAccs / NG;                   // steps from a release to its reuse
+    static constexpr int kGroupBars = kAccs > 4 ? kAccs : 4;  // group barriers (see the kernel)
     static constexpr int kWOff = kXStages * kX;
     static constexpr int kBarOff = kWOff + kWStages * kW;
-    static constexpr int kGroupBars = 4;                      // at least kAccs and NG - 1
-    static constexpr int kBars = 2 * kWStages + 2 * kXStages + 2 + kGroupBars + kAccs + 1;
+    static constexpr int kBars = 2 * kWStages + 2 * kXStages + kGroupBars + kAccs + 1;
     static constexpr int kMiscOff = kBarOff + kBars * 8;
     static constexpr int kAlloc = kMiscOff + 16 + 1024;       // slack to align the base to 1 KB
     static constexpr int kFoldHalves = NT <= 32 ? 1 : 2;      // fold warps per lane quarter
@@ -175,26 +180,20 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
 }
 
 // 16 bytes of x to shared memory, the first `bytes` of them (0, 2, .. 16) from memory, the rest 0.
-__device__ __forceinline__ void w4_stage16(uint32_t dst, const __nv_bfloat16* src, int bytes,
-                                           bool wide) {
-    if (wide) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-                     "r"(bytes) : "memory");
-    } else {
-        uint32_t v[4] = {0u, 0u, 0u, 0u};
+__device__ __forceinline__ void w4_stage16(uint32_t dst, const __nv_bfloat16* src, int bytes) {
+    uint32_t v[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (2 * i < bytes)
-                v[i >> 1] |= (uint32_t)__bfloat16_as_ushort(src[i]) << (16 * (i & 1));
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v[0]), "r"(v[1]),
-                     "r"(v[2]), "r"(v[3]) : "memory");
-    }
+    for (int i = 0; i < 8; ++i)
+        if (2 * i < bytes) v[i >> 1] |= (uint32_t)__bfloat16_as_ushort(src[i]) << (16 * (i & 1));
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]) : "memory");
 }
 
 // NT: token tile (16, 32 or 64); NG: groups per K step; ZP: zero points given; FP16: scales are
 // fp16, else bf16.
 template <int NT, int NG, bool ZP, bool FP16>
-__global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
+__global__ void __launch_bounds__(kW4Threads, 2)
+w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
     using L = W4Smem<NT, NG>;
     constexpr int WS = L::kWStages, XS = L::kXStages, DB = L::kAccs;
     constexpr int FH = L::kFoldHalves, SETS = L::kWidenSets;
@@ -214,29 +213,22 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
 
     const uint32_t bar_full = base + L::kBarOff;         // weights of a step have landed
     const uint32_t bar_empty = bar_full + WS * 8;        // ... and are used up
-    const uint32_t bar_xfull = bar_empty + WS * 8;       // activations of a step are there
-    const uint32_t bar_done = bar_xfull + XS * 8;        // a step's MMAs have finished
-    const uint32_t bar_afull = bar_done + XS * 8;        // a step is widened
-    const uint32_t bar_dfull = bar_afull + 2 * 8;        // a group that is not its step's last is summed
-    const uint32_t bar_dempty = bar_dfull + L::kGroupBars * 8;
-    const uint32_t bar_drain = bar_dempty + DB * 8;
+    const uint32_t bar_ready = bar_empty + WS * 8;       // a step's operands (and accumulators) are ready
+    const uint32_t bar_done = bar_ready + XS * 8;        // a step's MMAs have finished
+    const uint32_t bar_group = bar_done + XS * 8;        // a group that is not its step's last is summed
+    const uint32_t bar_free = bar_group + L::kGroupBars * 8;  // an accumulator may be overwritten
+    const uint32_t bar_drain = bar_free + DB * 8;
     volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(gbase + L::kMiscOff);
     volatile uint32_t* abort_flag = misc + 1;
 
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < WS; ++i) {
-            mbar_init(bar_full + 8 * i, 1);
-            mbar_init(bar_empty + 8 * i, 4 + 4 * FH);
-        }
-        for (int i = 0; i < XS; ++i) {
-            mbar_init(bar_xfull + 8 * i, 2);
-            mbar_init(bar_done + 8 * i, 1);
-        }
-        for (int i = 0; i < 2; ++i) mbar_init(bar_afull + 8 * i, 4);
-        for (int i = 0; i < L::kGroupBars; ++i) mbar_init(bar_dfull + 8 * i, 1);
-        for (int i = 0; i < DB; ++i) mbar_init(bar_dempty + 8 * i, 4 * FH);
-        mbar_init(bar_drain, 1);
-        *abort_flag = 0u;
+    if (threadIdx.x < L::kBars) {
+        const int i = threadIdx.x;
+        int count = 1;
+        if (i >= WS && i < 2 * WS) count = 4 + 4 * FH;
+        else if (i >= 2 * WS && i < 2 * WS + XS) count = 2 + 4 + (L::kStepRelease ? 4 * FH : 0);
+        else if (i >= 2 * WS + 2 * XS + L::kGroupBars && i < L::kBars - 1) count = 4 * FH;
+        mbar_init(bar_full + 8 * i, count);
+        if (i == 0) *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -256,12 +248,11 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
     constexpr int kFold0 = 4, kWiden0 = 4 + 4 * FH;
     // A group's barrier completes once per round of the index that names it, and no second time
     // before the fold warps have seen the first: by accumulator where a round of the DB
-    // accumulators holds two steps' groups, else by the group's place in its step (the MMAs are
-    // never a whole step of groups ahead of the fold warps there).
-    constexpr bool kByAcc = DB == 4 && NG == 2;
-    static_assert(kByAcc || DB <= NG || NG == 1, "group barriers");
-    // The done barrier of a step comes round after XS steps; fold warps lag by at most DB groups.
-    static_assert(XS >= DB && XS >= 3, "done barriers");
+    // accumulators is whole steps, else by the group's place in its step (the MMAs are never a
+    // step of groups ahead of the fold warps there).
+    constexpr bool kByAcc = DB >= NG;
+    // A step's barriers come round after XS steps; the MMAs are never that far ahead.
+    static_assert(XS >= DB && XS >= L::kLag && XS >= 3, "step barriers");
     if (warp == 0) {
         if (lane == 0) {
             // weights do not depend on the previous launch: no wait for it
@@ -286,9 +277,6 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
                     bulk_load_hint(dst + kW4StepBytes + L::kScale, zeros + (int64_t)i * L::kZero,
                                    L::kZero, bar, policy);
             }
-            if (i < n)  // stopped: the copies in flight must land before the CTA goes
-                for (int j = i > WS ? i - WS : 0; j < i; ++j)
-                    w4_wait(bar_full + 8 * (j % WS), (j / WS) & 1);
         }
     } else if (warp == 1) {
         // the whole warp walks the loop, so that descriptors stay in uniform registers
@@ -297,16 +285,17 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
         bool ok = true;
         int xs = 0, xph = 0, db = 0, dph = 1;
 #pragma unroll 1
-        for (int i = 0; i < n && ok; ++i) {
-            const uint32_t ab = i & 1;
-            ok = w4_wait(bar_xfull + 8 * xs, xph) && w4_wait(bar_afull + 8 * ab, (i >> 1) & 1);
+        for (int i = 0; i < n; ++i) {
+            ok = w4_wait(bar_ready + 8 * xs, xph);
             if (!ok) break;
             const uint64_t bdesc = sw128_desc(base + xs * L::kX);
-            const uint32_t ta = tmem + ab * 64;
+            const uint32_t ta = tmem + (i & 1) * 64;
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
-                ok = w4_wait(bar_dempty + 8 * db, dph);  // passes at once for the first DB groups
-                if (!ok) break;
+                if (!L::kStepRelease) {
+                    ok = w4_wait(bar_free + 8 * db, dph);  // passes at once for the first DB groups
+                    if (!ok) break;
+                }
                 tc_fence_after();
                 if (leader) {
 #pragma unroll
@@ -316,7 +305,7 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
                                   bdesc + (((kk >> 2) * (NT * 128) + 32 * (kk & 3)) >> 4), idesc,
                                   k > 0);
                     }
-                    tc_commit(j == NG - 1 ? bar_done + 8 * xs : bar_dfull + 8 * (kByAcc ? db : j));
+                    tc_commit(j == NG - 1 ? bar_done + 8 * xs : bar_group + 8 * (kByAcc ? db : j));
                 }
                 __syncwarp();
                 if (++db == DB) {
@@ -324,6 +313,7 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
                     dph ^= 1;
                 }
             }
+            if (!ok) break;
             if (++xs == XS) {
                 xs = 0;
                 xph ^= 1;
@@ -335,16 +325,35 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
             __syncwarp();
             w4_wait(bar_drain, 0);
         }
+    } else if (warp < kFold0 && a.wide_x) {
+        if (warp == 2 && lane == 0) {
+            griddep_wait();  // x is the previous launch's
+            int xs = 0, ph = 1;
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) {
+                if (!w4_wait(bar_done + 8 * xs, ph)) {  // passes at once for the first XS steps
+                    *abort_flag = 1u;
+                    break;
+                }
+                const uint32_t bar = bar_ready + 8 * xs, dst = base + xs * L::kX;
+                mbar_expect_tx(bar, L::kX);
+                mbar_arrive(bar);  // (two arrivals, as the copying warps make)
+                tma_load_2d(dst, &tmap_x, bar, (k_begin + i) * 128, m0);
+                tma_load_2d(dst + NT * 128, &tmap_x, bar, (k_begin + i) * 128 + 64, m0);
+                if (++xs == XS) {
+                    xs = 0;
+                    ph ^= 1;
+                }
+            }
+        }
     } else if (warp < kFold0) {
-        // 64 threads: piece c (8 wide) of tokens r, r + 4, ..; LEAD steps ahead of the MMAs
-        constexpr int LEAD = XS - 2;
-        griddep_wait();  // x is the previous launch's
+        griddep_wait();
+        // 64 threads: piece c (8 wide) of tokens r, r + 4, ..
         const int tid = threadIdx.x - 64, c = tid & 15, r = tid >> 4;
         const __nv_bfloat16* src = a.x + (int64_t)(m0 + r) * a.ldx + k_begin * 128 + c * 8;
         const uint32_t dst = base + (c >> 3) * (NT * 128) + r * 128;
         const uint32_t sw0 = ((c & 7) ^ r) << 4, sw1 = ((c & 7) ^ (r + 4)) << 4;
         const int64_t row4 = 4 * a.ldx;
-        const bool wide = a.wide_x != 0;
         const int left = a.K - k_begin * 128 - c * 8;  // elements from the first step's piece on
         auto issue = [&](int i, int xs) {
             const int bytes = 2 * min(max(left - i * 128, 0), 8);
@@ -354,34 +363,23 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
             // columns of tokens past mcount stay as they are: they only reach sums never stored
 #pragma unroll 1
             for (int m = r; m < mcount; m += 4, p += next, d += 512)
-                w4_stage16(d + ((m & 4) ? sw1 : sw0), p, bytes, wide);
-            asm volatile("cp.async.commit_group;" ::: "memory");
+                w4_stage16(d + ((m & 4) ? sw1 : sw0), p, bytes);
         };
         bool ok = true;
-        for (int i = 0; i < min(n, LEAD); ++i) issue(i, i);
-        for (int i = n; i < LEAD; ++i) asm volatile("cp.async.commit_group;" ::: "memory");
-        int xs = 0, ahead = LEAD, aph = 1;  // aph: parity of step i + LEAD's predecessor in its slot
+        int xs = 0, ph = 1;
 #pragma unroll 1
         for (int i = 0; i < n; ++i) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(LEAD - 1) : "memory");
+            ok = __all_sync(0xffffffffu, w4_wait(bar_done + 8 * xs, ph));
+            if (!ok) break;
+            issue(i, xs);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_xfull + 8 * xs);
-            if (++xs == XS) xs = 0;
-            if (i + LEAD < n) {
-                ok = w4_wait(bar_done + 8 * ahead, aph);  // passes at once for the first XS steps
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                issue(i + LEAD, ahead);
-            } else {
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            }
-            if (++ahead == XS) {
-                ahead = 0;
-                aph ^= 1;
+            if (lane == 0) mbar_arrive(bar_ready + 8 * xs);
+            if (++xs == XS) {
+                xs = 0;
+                ph ^= 1;
             }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
         if (!ok) *abort_flag = 1u;
     } else if (warp < kWiden0) {
         const int quarter = warp & 3, half = (warp - kFold0) >> 2;
@@ -392,7 +390,9 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
 #pragma unroll
         for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
         bool ok = true;
-        int st = 0, wph = 0, xs = 0, xph = 0, db = 0, dph = 0;
+        int st = 0, wph = 0, xs = 0, xph = 0, db = 0, dph = 0, later = L::kLag % XS;
+        if (L::kStepRelease && lane == 0)  // the first steps find every accumulator free
+            for (int i = 0; i < L::kLag; ++i) mbar_arrive(bar_ready + 8 * i);
 #pragma unroll 1
         for (int i = 0; i < n && ok; ++i) {
             ok = __all_sync(0xffffffffu, w4_wait(bar_full + 8 * st, wph));
@@ -415,8 +415,8 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
             for (int j = 0; j < NG; ++j) {
                 ok = __all_sync(0xffffffffu,
                                 j == NG - 1 ? w4_wait(bar_done + 8 * xs, xph)
-                                            : w4_wait(bar_dfull + 8 * (kByAcc ? db : j),
-                                                        kByAcc ? dph : i & 1));
+                                            : w4_wait(bar_group + 8 * (kByAcc ? db : j),
+                                                      kByAcc ? dph : i & 1));
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll
@@ -427,12 +427,19 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
                     for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(s[j], v[e], acc[c + e]);
                 }
                 tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar_dempty + 8 * db);
+                if (!L::kStepRelease) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_free + 8 * db);
+                }
                 if (++db == DB) {
                     db = 0;
                     dph ^= 1;
                 }
+            }
+            if (L::kStepRelease) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_ready + 8 * later);
+                if (++later == XS) later = 0;
             }
             if (++xs == XS) {
                 xs = 0;
@@ -452,6 +459,7 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
         const int row = quarter * 32 + lane;
         bool ok = true;
         int st = set, wph = 0, xs = XS - 2 + set, xph = 1;  // xs, xph: of step i - 2
+        int ready = set;
 #pragma unroll 1
         for (int i = set; i < n; i += SETS) {
             const uint32_t ab = i & 1;
@@ -491,7 +499,8 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_afull + 8 * ab);
+            if (lane == 0) mbar_arrive(bar_ready + 8 * ready);
+            if ((ready += SETS) >= XS) ready -= XS;
             if ((st += SETS) >= WS) {
                 st -= WS;
                 wph ^= 1;
@@ -506,6 +515,11 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Args a) {
 
     __syncwarp();
     tc_fence_before();
+    __syncthreads();
+    if (*abort_flag && threadIdx.x == 0) {  // copies in flight must land before the CTA goes: they
+        const uint64_t t0 = global_ns();    // take microseconds, and get a millisecond
+        while (global_ns() - t0 < 1000000ull) __nanosleep(1000);
+    }
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
@@ -570,11 +584,14 @@ static int w4_launch(const W4Args& a, cudaStream_t s) {
     }
     const int tiles = (a.N + kW4Rows - 1) / kW4Rows, mt = (a.M + NT - 1) / NT;
     // K is split while the CTAs still fit the GPU at once and keep two steps each
-    int S = (int)min((int64_t)kW4MaxCluster, (int64_t)2 * sms[dev] / ((int64_t)tiles * mt));
+    int S = (int)min((int64_t)kW4MaxCluster, (int64_t)256 / ((int64_t)tiles * mt));
     S = max(1, min(S, a.KB / 2));
 #ifdef W4_TUNE
     if (w4_tune_s) S = min(w4_tune_s, a.KB);
 #endif
+    CUtensorMap mx{};
+    if (a.wide_x && (get_encoder() != NK_OK || make_map(&mx, a.x, a.M, a.K, a.ldx, NT) != NK_OK))
+        return NK_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles * S, mt);
     cfg.blockDim = dim3(kW4Threads);
@@ -589,7 +606,7 @@ static int w4_launch(const W4Args& a, cudaStream_t s) {
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = S > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? NK_OK : NK_ERR_CUDA;
+    return cudaLaunchKernelEx(&cfg, kernel, mx, a) == cudaSuccess ? NK_OK : NK_ERR_CUDA;
 }
 
 template <int NT, int NG>
@@ -642,7 +659,7 @@ extern "C" int nk_gemm_w4(const void* x, int64_t ldx, const void* codes, const v
         return NK_ERR_ALIGN;
     W4Args a{};
     a.x = static_cast<const __nv_bfloat16*>(x);
-    a.ldx = ldx;
+    a.ldx = M == 1 ? (K + 7) / 8 * 8 : ldx;  // (one row: any stride)
     a.codes = static_cast<const uint8_t*>(codes);
     a.scales = static_cast<const uint8_t*>(scales);
     a.zeros = static_cast<const uint8_t*>(zeros);
@@ -652,7 +669,7 @@ extern "C" int nk_gemm_w4(const void* x, int64_t ldx, const void* codes, const v
     a.N = N;
     a.K = K;
     a.KB = (K + 127) / 128;
-    a.wide_x = ((uintptr_t)x & 15u) == 0 && ldx % 8 == 0;
+    a.wide_x = ((uintptr_t)x & 15u) == 0 && a.ldx % 8 == 0;
     const bool fp16 = scale_type == NK_W4_SCALE_FP16;
     cudaStream_t s = (cudaStream_t)stream;
     if (M <= 16) return w4_dispatch<16>(a, group, fp16, s);
