@@ -221,16 +221,34 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
     volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(gbase + L::kMiscOff);
     volatile uint32_t* abort_flag = misc + 1;
 
-    if (threadIdx.x < L::kBars) {
-        const int i = threadIdx.x;
-        int count = 1;
-        if (i >= WS && i < 2 * WS) count = 4 + 4 * FH;
-        else if (i >= 2 * WS && i < 2 * WS + XS) count = 2 + 4 + (L::kStepRelease ? 4 * FH : 0);
-        else if (i >= 2 * WS + 2 * XS + L::kGroupBars && i < L::kBars - 1) count = 4 * FH;
-        mbar_init(bar_full + 8 * i, count);
-        if (i == 0) *abort_flag = 0u;
+    // Weights do not depend on the previous launch: the first steps' are on their way before tensor
+    // memory is allocated and before the wait for that launch.
+    const uint64_t policy = l2_evict_first_policy();
+    auto load_step = [&](int i, int st) {
+        const int64_t at = (int64_t)tile * a.KB + k_begin + i;
+        const uint32_t dst = base + L::kWOff + st * L::kW, bar = bar_full + 8 * st;
+        mbar_expect_tx(bar, kW4StepBytes + L::kScale + (ZP ? L::kZero : 0));
+        bulk_load_hint(dst, a.codes + at * kW4StepBytes, kW4StepBytes, bar, policy);
+        bulk_load_hint(dst + kW4StepBytes, a.scales + at * L::kScale, L::kScale, bar, policy);
+        if (ZP)
+            bulk_load_hint(dst + kW4StepBytes + L::kScale, a.zeros + at * L::kZero, L::kZero, bar,
+                           policy);
+    };
+    if (warp == 0) {
+        for (int i = lane; i < L::kBars; i += 32) {
+            int count = 1;
+            if (i >= WS && i < 2 * WS) count = 4 + 4 * FH;
+            else if (i >= 2 * WS && i < 2 * WS + XS) count = 2 + 4 + (L::kStepRelease ? 4 * FH : 0);
+            else if (i >= 2 * WS + 2 * XS + L::kGroupBars && i < L::kBars - 1) count = 4 * FH;
+            mbar_init(bar_full + 8 * i, count);
+        }
+        if (lane == 0) *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0)
+            for (int i = 0; i < min(n, WS); ++i) load_step(i, i);
+        __syncwarp();
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -255,27 +273,18 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
     static_assert(XS >= DB && XS >= L::kLag && XS >= 3, "step barriers");
     if (warp == 0) {
         if (lane == 0) {
-            // weights do not depend on the previous launch: no wait for it
-            const uint64_t policy = l2_evict_first_policy();
-            const int64_t at = (int64_t)tile * a.KB + k_begin;
-            const uint8_t* codes = a.codes + at * kW4StepBytes;
-            const uint8_t* scales = a.scales + at * L::kScale;
-            const uint8_t* zeros = ZP ? a.zeros + at * L::kZero : nullptr;
-            int i = 0;
-            for (; i < n; ++i) {
-                const int st = i % WS;
-                if (i >= WS && !w4_wait(bar_empty + 8 * st, (i / WS - 1) & 1)) {
+            int st = 0, ph = 0;
+#pragma unroll 1
+            for (int i = WS; i < n; ++i) {
+                if (!w4_wait(bar_empty + 8 * st, ph)) {
                     *abort_flag = 1u;
                     break;
                 }
-                const uint32_t dst = base + L::kWOff + st * L::kW, bar = bar_full + 8 * st;
-                mbar_expect_tx(bar, kW4StepBytes + L::kScale + (ZP ? L::kZero : 0));
-                bulk_load_hint(dst, codes + (int64_t)i * kW4StepBytes, kW4StepBytes, bar, policy);
-                bulk_load_hint(dst + kW4StepBytes, scales + (int64_t)i * L::kScale, L::kScale, bar,
-                               policy);
-                if (ZP)
-                    bulk_load_hint(dst + kW4StepBytes + L::kScale, zeros + (int64_t)i * L::kZero,
-                                   L::kZero, bar, policy);
+                load_step(i, st);
+                if (++st == WS) {
+                    st = 0;
+                    ph ^= 1;
+                }
             }
         }
     } else if (warp == 1) {
