@@ -241,10 +241,12 @@ constexpr int kQ8Unit = 64;                 // slots per unit, 16 per warp
 constexpr int kQ8AttnThreads = 128;
 constexpr int kQ8Stages = 4;                // units in flight per warp
 constexpr int kQ8WarpStage = 2 * 16 * 128;  // K and V rows of 16 slots
-constexpr int kQ8AttnSmem = kQ8Stages * 4 * kQ8WarpStage;  // 64 KB
+constexpr int kQ8Ring = kQ8Stages * 4 * kQ8WarpStage;         // 64 KB
+constexpr int kQ8AttnSmem = kQ8Ring + 4 * kQ8Stages * 8;      // and each stage's two scales
 constexpr int kQ8MaxGrid = 148 * 4;
-constexpr int kQ8PartFloats = kHeadDim + 4; // O, m, my, l, unused
+constexpr int kQ8PartFloats = kHeadDim + 4; // O, then m, my, l
 constexpr float kQ8Shift = 15.f;            // probabilities are held times 2^15
+constexpr int kQ8MergeWarps = 8;
 
 struct Q8AttnArgs {
     const __nv_bfloat16* q;
@@ -253,9 +255,10 @@ struct Q8AttnArgs {
     const int64_t* position; int per_sequence;
     __nv_bfloat16* out;
     float* part;                 // [grid][2][rows][kQ8PartFloats]
-    int batch, tokens, hq, hkv, G, capacity, block, blocks;
+    int batch, tokens, hq, hkv, G, capacity, lg_block, blocks;
     int rows, row_blocks;        // query rows of a CTA (8 NT), row blocks of T * G rows
     int grid;                    // CTAs of the first launch
+    int lg_wpr;                  // merge: log2 of the warps that share a row
     int64_t cb, ch, cs;
     float scale_log2;            // softmax scale times log2(e)
 };
@@ -281,150 +284,176 @@ __device__ __forceinline__ uint32_t movm_t(uint32_t v) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t v16) {  // low half of v16
-    uint32_t h;
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}"
-        : "=r"(h) : "r"(v16));
-    return h;
-}
-__device__ __forceinline__ uint32_t e4m3x2_f16x2_hi(uint32_t v32) {
-    uint32_t h;
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}"
-        : "=r"(h) : "r"(v32));
-    return h;
+// Four e4m3 codes as two f16 pairs (codes 0, 1 and 2, 3).
+__device__ __forceinline__ void e4m3x4_f16(uint32_t v, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-__device__ __forceinline__ float ex2(float x) { return exp2f(x); }
+// 2^x and log2 x by the special-function unit (2^x: relative error 2^-22; results below 2^-126 are
+// 0; log2 of a power of two is off by 2^-22 of it at most: both far below the 2^-11 of the f16
+// probabilities).
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // Factor of a part with running maximum m where all parts have maximum M. A part that saw nothing
 // (m = -inf) has sums of 0, or NaN if what it saw was NaN: 1 keeps both.
 __device__ __forceinline__ float q8_weight(float m, float M) {
     return m == -INFINITY ? 1.f : ex2(m - M);
 }
 
-// Units of the launch, from the device positions: s_end[b] = units of sequences 0 .. b, of one
-// (kv head, row block). Every thread of the CTA calls it.
-__device__ __forceinline__ void q8_units(const Q8AttnArgs& a, int* s_end) {
-    for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
-        const int64_t p = q8_position(a.position, a.per_sequence, b, a.tokens, a.capacity);
-        s_end[b] = p < 0 ? 0 : (int)((p + a.tokens + kQ8Unit - 1) / kQ8Unit);
-    }
-    __syncthreads();
-    if (threadIdx.x < 32) {  // running sum, 32 sequences at a time
-        int base = 0;
-        for (int b0 = 0; b0 < a.batch; b0 += 32) {
-            const int b = b0 + threadIdx.x;
-            int x = b < a.batch ? s_end[b] : 0;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, off);
-                if ((int)threadIdx.x >= off) x += y;
-            }
-            x += base;
-            if (b < a.batch) s_end[b] = x;
-            base = __shfl_sync(0xffffffffu, x, 31);
-        }
-    }
-    __syncthreads();
+// Units of sequence b, of one (kv head, row block).
+__device__ __forceinline__ int q8_seq_units(const Q8AttnArgs& a, int b) {
+    const int64_t p = q8_position(a.position, a.per_sequence, b, a.tokens, a.capacity);
+    return p < 0 ? 0 : ((int)p + a.tokens + kQ8Unit - 1) / kQ8Unit;
 }
 
-// The partition of U units over G CTAs (begin(c) = floor(U c / G)) and its inverse.
-__device__ __forceinline__ int64_t q8_begin(int64_t U, int G, int c) { return U * c / G; }
-__device__ __forceinline__ int q8_cta_of(int64_t U, int G, int64_t u) {
-    return (int)(((u + 1) * G + U - 1) / U - 1);
-}
+// The partition of U units over G <= U CTAs, q = U / G or one more each, and its inverse.
+struct Q8Split {
+    uint32_t q, r;
+    __device__ Q8Split(uint32_t U, uint32_t G) : q(U / G), r(U - U / G * G) {}
+    __device__ uint32_t begin(uint32_t c) const { return c * q + min(c, r); }
+    __device__ uint32_t cta_of(uint32_t u) const {
+        const uint32_t t = r * (q + 1);
+        return u < t ? u / (q + 1) : r + (u - t) / q;
+    }
+};
 
 template <int NT>
 __global__ void __launch_bounds__(kQ8AttnThreads, NT <= 2 ? 3 : 2)
 q8_attn_kernel(const Q8AttnArgs a) {
     extern __shared__ __align__(1024) uint8_t q8_smem[];
-    __shared__ int s_end[NK_Q8_MAX_BATCH];
+    __shared__ int s_end[NK_Q8_MAX_BATCH];              // running sum of the sequences' units
     __shared__ float s_stat[4][8 * NT][4];
+    __shared__ uint2 s_q[NT > 1 ? NT * 8 * 32 : 1];     // Q^T operand, shared by the warps
     if (threadIdx.x == 0) griddep_launch_dependents();
     griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    q8_units(a, s_end);
-    const int per_b = a.hkv * a.row_blocks;                 // pairs per sequence
-    const int64_t U = (int64_t)s_end[a.batch - 1] * per_b;
-    if (blockIdx.x == 0) {
-        for (int b = threadIdx.x; b < a.batch; b += blockDim.x)
+    if (warp == 0) {  // 128 sequences at a time, their positions read together
+        int base = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += 128) {
+            int x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int b = b0 + 32 * i + lane;
+                x[i] = b < a.batch ? q8_seq_units(a, b) : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int b = b0 + 32 * i + lane;
+                if (b0 + 32 * i >= a.batch) break;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, x[i], off);
+                    if (lane >= off) x[i] += y;
+                }
+                x[i] += base;
+                if (b < a.batch) s_end[b] = x[i];
+                base = __shfl_sync(0xffffffffu, x[i], 31);
+            }
+        }
+    } else if (blockIdx.x == 0 && warp == 1) {
+        for (int b = lane; b < a.batch; b += 32)
             if (a.position[a.per_sequence ? b : 0] > (int64_t)a.capacity - a.tokens)
                 atomicExch(&g_error, NK_ERR_RANGE);
     }
-    const int G = (int)min((int64_t)a.grid, U);             // no CTA of the partition is empty
-    if ((int)blockIdx.x >= G) return;
-    int64_t u = q8_begin(U, G, blockIdx.x);
-    const int64_t u_end = q8_begin(U, G, blockIdx.x + 1);
-    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(q8_smem)) +
-                          warp * (kQ8Stages * kQ8WarpStage);
+    __syncthreads();
+    const uint32_t per_b = a.hkv * a.row_blocks;            // pairs per sequence
+    const uint32_t U = s_end[a.batch - 1] * per_b;
+    const uint32_t G = min((uint32_t)a.grid, U);            // no CTA of the partition is empty
+    if (blockIdx.x >= G) return;
+    const Q8Split split(U, G);
+    uint32_t u = split.begin(blockIdx.x);
+    const uint32_t u_end = split.begin(blockIdx.x + 1);
+    const uint32_t smem0 = static_cast<uint32_t>(__cvta_generic_to_shared(q8_smem));
+    const uint32_t ring = smem0 + warp * (kQ8Stages * kQ8WarpStage);
+    const uint32_t s_scale = smem0 + kQ8Ring + warp * (kQ8Stages * 8);
 
     while (u < u_end) {
         // the pair of unit u: sequence b, kv head h, row block rb; its units [p0, p0 + n)
         int lo = 0, hi = a.batch - 1;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if ((int64_t)s_end[mid] * per_b > u) hi = mid; else lo = mid + 1;
+            if (s_end[mid] * per_b > u) hi = mid; else lo = mid + 1;
         }
-        const int b = lo;
-        const int64_t before = b > 0 ? (int64_t)s_end[b - 1] * per_b : 0;
-        const int n = s_end[b] - (b > 0 ? s_end[b - 1] : 0);
-        const int pr = (int)((u - before) / n);
-        const int64_t p0 = before + (int64_t)pr * n;
+        const int b = lo, first = b > 0 ? s_end[b - 1] : 0;
+        const uint32_t n = s_end[b] - first, before = first * per_b;
+        const uint32_t pr = (u - before) / n, p0 = before + pr * n;
         const int h = pr / a.row_blocks, rb = pr - h * a.row_blocks;
-        const int c0 = (int)(u - p0), c1 = (int)(min(u_end, p0 + n) - p0);
-        const int64_t pos = q8_position(a.position, a.per_sequence, b, a.tokens, a.capacity);
-        const int64_t len = pos + a.tokens;
+        const int c0 = u - p0, c1 = min(u_end, p0 + n) - p0;
+        const int pos = (int)a.position[a.per_sequence ? b : 0];
+        const int len = pos + a.tokens;
 
-        const uint8_t* kb = a.k + (int64_t)b * a.cb + (int64_t)h * a.ch;
-        const uint8_t* vb = a.v + (int64_t)b * a.cb + (int64_t)h * a.ch;
-        const float* ksb = a.ks + ((int64_t)b * a.hkv + h) * a.blocks;
-        const float* vsb = a.vs + ((int64_t)b * a.hkv + h) * a.blocks;
-
-        // 16 slots of a unit: eight 16-byte pieces a row, piece c at c ^ (row & 7)
-        auto issue = [&](int c) {
-            if (c < c1) {
-                const uint32_t dst = ring + (c % kQ8Stages) * kQ8WarpStage;
-                const int64_t j0 = (int64_t)c * kQ8Unit + warp * 16;
+        // 16 slots of a unit: eight 16-byte pieces a row, piece c at c ^ (row & 7); this lane
+        // copies piece lane % 8 of rows lane / 8 + 0, 4, 8, 12
+        int slot = c0 * kQ8Unit + warp * 16 + (lane >> 3);
+        const int64_t pair = (int64_t)b * a.cb + (int64_t)h * a.ch;
+        const uint8_t* kp = a.k + pair + (int64_t)slot * a.cs + (lane & 7) * 16;
+        const uint8_t* vp = a.v + pair + (int64_t)slot * a.cs + (lane & 7) * 16;
+        const float* sp = (lane & 1 ? a.vs : a.ks) + ((int64_t)b * a.hkv + h) * a.blocks;
+        const uint32_t d0 = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);
+        const uint32_t d1 = d0 ^ (4 << 4);  // rows 4 on: (row & 7) has bit 2 set
+        const int64_t row4 = 4 * a.cs, next = kQ8Unit * a.cs;
+        int fill = c0;
+        auto issue = [&]() {
+            if (fill < c1) {
+                const uint32_t st = fill & (kQ8Stages - 1);
+                const uint32_t dst = ring + st * kQ8WarpStage;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int idx = i * 32 + lane, row = idx >> 3, piece = idx & 7;
-                    const bool ok = j0 + row < len;
-                    const int64_t off = ok ? (j0 + row) * a.cs + piece * 16 : 0;
-                    const uint32_t d = dst + row * 128 + ((piece ^ (row & 7)) * 16);
-                    cp_async<16>(d, kb + off, ok);
-                    cp_async<16>(d + 16 * 128, vb + off, ok);
+                    const bool ok = slot + 4 * i < len;
+                    const uint32_t d = dst + (i & 1 ? d1 : d0) + i * 512;
+                    cp_async<16>(d, ok ? kp + i * row4 : a.k, ok);
+                    cp_async<16>(d + 16 * 128, ok ? vp + i * row4 : a.v, ok);
                 }
+                const int s0 = fill * kQ8Unit + warp * 16;
+                if (lane < 2 && s0 < len)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(
+                                     s_scale + st * 8 + lane * 4), "l"(sp + (s0 >> a.lg_block))
+                                 : "memory");
+                slot += kQ8Unit;
+                kp += next;
+                vp += next;
+                ++fill;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
-        for (int i = 0; i < kQ8Stages - 1; ++i) issue(c0 + i);
+        for (int i = 0; i < kQ8Stages - 1; ++i) issue();
 
         // Q^T operand: column g of tile nt is query row 8 nt + g; dims 16 s + 4 t .. + 3 of step s
-        uint32_t qf[NT][8][2];
+        uint2 qf[NT > 1 ? 1 : 8];
         float qs[NT][2];     // 2^-shift of rows 8 nt + 2t, + 1, times the softmax scale
         int last[NT][2];     // last slot those rows see, relative to pos (-1: no such row)
+        const int total_rows = a.tokens * a.G;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int r = rb * a.rows + 8 * nt + g;
-            const bool ok = r < a.tokens * a.G;
+            const bool ok = r < total_rows;
             const int tok = ok ? r / a.G : 0, hh = ok ? r - tok * a.G : 0;
             const __nv_bfloat16* src =
-                a.q + (((int64_t)b * a.tokens + tok) * a.hq + (int64_t)h * a.G + hh) * kHeadDim;
-            float x[8][4], m = 0.f;
+                a.q + (((int64_t)b * a.tokens + tok) * a.hq + (int64_t)h * a.G + hh) * kHeadDim + 4 * t;
+            uint2 w[8];
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                uint2 w = make_uint2(0u, 0u);
-                if (ok) w = *reinterpret_cast<const uint2*>(src + 16 * s + 4 * t);
-                x[s][0] = bf16lo(w.x); x[s][1] = bf16hi(w.x);
-                x[s][2] = bf16lo(w.y); x[s][3] = bf16hi(w.y);
+            for (int s = 0; s < 8; ++s)
+                w[s] = ok ? *reinterpret_cast<const uint2*>(src + 16 * s) : make_uint2(0u, 0u);
+            float m = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(x[s][i]));
-            }
+            for (int s = 0; s < 8; ++s)
+                m = fmaxf(m, fmaxf(fmaxf(fabsf(bf16lo(w[s].x)), fabsf(bf16hi(w[s].x))),
+                                   fmaxf(fabsf(bf16lo(w[s].y)), fabsf(bf16hi(w[s].y)))));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
             // largest magnitude to [2^12, 2^13): a bf16 value keeps its 8 bits down to 2^-29 of it
@@ -434,16 +463,19 @@ q8_attn_kernel(const Q8AttnArgs a) {
             const float down = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
-                qf[nt][s][0] = pack_f16x2(x[s][0] * up, x[s][1] * up);
-                qf[nt][s][1] = pack_f16x2(x[s][2] * up, x[s][3] * up);
+                const uint2 f = make_uint2(pack_f16x2(bf16lo(w[s].x) * up, bf16hi(w[s].x) * up),
+                                           pack_f16x2(bf16lo(w[s].y) * up, bf16hi(w[s].y) * up));
+                if (NT == 1) qf[s] = f;
+                else if ((nt & 3) == warp % NT || NT == 1) s_q[(nt * 8 + s) * 32 + lane] = f;
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 qs[nt][i] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + i)) * a.scale_log2;
                 const int rr = rb * a.rows + 8 * nt + 2 * t + i;
-                last[nt][i] = rr < a.tokens * a.G ? rr / a.G : -1;
+                last[nt][i] = rr < total_rows ? rr / a.G : -1;
             }
         }
+        if (NT > 1) __syncthreads();
 
         float m[NT][2], my[NT][2], l[NT][2], o[8][NT][4];
 #pragma unroll
@@ -455,85 +487,115 @@ q8_attn_kernel(const Q8AttnArgs a) {
         }
 
         // ldmatrix rows: matrix mi = lane / 8 = (slots half mi & 1, piece + (mi >> 1)), row lane % 8
-        const int mrow = (lane >> 3 & 1) * 8 + (lane & 7), mpiece = lane >> 4;
+        const uint32_t mrow = ((lane >> 3) & 1) * 8 + (lane & 7), mpiece = lane >> 4;
+        const uint32_t mbase = ring + mrow * 128, mx7 = mrow & 7;
+#pragma unroll 1
         for (int c = c0; c < c1; ++c) {
-            issue(c + kQ8Stages - 1);
+            issue();
             asm volatile("cp.async.wait_group %0;" ::"n"(kQ8Stages - 1) : "memory");
             __syncwarp();
-            const uint32_t st = ring + (c % kQ8Stages) * kQ8WarpStage;
-            const int64_t j0 = (int64_t)c * kQ8Unit + warp * 16;
+            const uint32_t stage = c & (kQ8Stages - 1), st = mbase + stage * kQ8WarpStage;
+            const int j0 = c * kQ8Unit + warp * 16;
             if (j0 < len) {
-                const int blk = (int)(j0 / a.block);
-                const float k_scale = ksb[blk];
-                const float v_log2 = log2f(vsb[blk]);
+                float k_scale, v_scale;
+                asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(k_scale), "=f"(v_scale)
+                             : "r"(s_scale + stage * 8) : "memory");
+                const float v_log2 = lg2(v_scale);
                 float s[NT][4];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
                 for (int p = 0; p < 8; p += 2) {
                     uint32_t r[4];
-                    ldsm_x4(st + mrow * 128 + (((p + mpiece) ^ (mrow & 7)) * 16), r);
+                    ldsm_x4(st + (((p + mpiece) ^ mx7) << 4), r);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint32_t a0 = e4m3x2_f16x2(r[2 * i]), a2 = e4m3x2_f16x2_hi(r[2 * i]);
-                        const uint32_t a1 = e4m3x2_f16x2(r[2 * i + 1]),
-                                       a3 = e4m3x2_f16x2_hi(r[2 * i + 1]);
+                        uint32_t a0, a1, a2, a3;
+                        e4m3x4_f16(r[2 * i], a0, a2);
+                        e4m3x4_f16(r[2 * i + 1], a1, a3);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-                            mma_f16(s[nt], a0, a1, a2, a3, qf[nt][p + i][0], qf[nt][p + i][1]);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const uint2 f = NT == 1 ? qf[NT == 1 ? p + i : 0]
+                                                    : s_q[(nt * 8 + p + i) * 32 + lane];
+                            mma_f16(s[nt], a0, a1, a2, a3, f.x, f.y);
+                        }
                     }
                 }
                 // scores of slots j0 + g, j0 + 8 + g against rows 2t, 2t + 1 of each tile
-                const int rel = (int)(j0 - pos);  // slots are seen up to pos + last
+                const int rel = j0 - pos + g;           // slots are seen up to pos + last
+                const bool all_seen = j0 + 15 <= pos;   // by every row
+                float mx[NT][2];
+                bool grown = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float f = qs[nt][i] * k_scale;
+                        s[nt][i] *= f;
+                        s[nt][i + 2] *= f;
+                    }
+                    if (!all_seen) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (rel + (i >> 1) * 8 > last[nt][i & 1]) s[nt][i] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float x = fmaxf(s[nt][i], s[nt][i + 2]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        mx[nt][i] = x;
+                        grown |= x > m[nt][i] || x + v_log2 > my[nt][i];
+                    }
+                }
+                if (__any_sync(0xffffffffu, grown)) {  // a new maximum: rescale the sums
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float al[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float mn = fmaxf(m[nt][i], mx[nt][i]);
+                            const float yn = fmaxf(my[nt][i], mx[nt][i] + v_log2);
+                            l[nt][i] *= ex2(m[nt][i] - (mn == -INFINITY ? 0.f : mn));
+                            al[i] = ex2(my[nt][i] - (yn == -INFINITY ? 0.f : yn));
+                            m[nt][i] = mn;
+                            my[nt][i] = yn;
+                        }
+#pragma unroll
+                        for (int d = 0; d < 8; ++d) {
+                            o[d][nt][0] *= al[0];
+                            o[d][nt][1] *= al[1];
+                            o[d][nt][2] *= al[0];
+                            o[d][nt][3] *= al[1];
+                        }
+                    }
+                }
                 uint32_t pf[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float x[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[i] = s[nt][i] * (qs[nt][i & 1] * k_scale);
-                        if (rel + g + (i >> 1) * 8 > last[nt][i & 1]) x[i] = -INFINITY;
-                    }
-                    float f[2][2], al[2];
+                    float f[2][2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float mx = fmaxf(x[i], x[i + 2]);
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float mn = fmaxf(m[nt][i], mx);
-                        const float ref = mn == -INFINITY ? 0.f : mn;
-                        l[nt][i] = l[nt][i] * ex2(m[nt][i] - ref) + ex2(x[i] - ref) +
-                                   ex2(x[i + 2] - ref);
-                        m[nt][i] = mn;
-                        const float yn = fmaxf(my[nt][i], mx + v_log2);
-                        const float yref = yn == -INFINITY ? 0.f : yn;
-                        al[i] = ex2(my[nt][i] - yref);
-                        my[nt][i] = yn;
-                        f[0][i] = ex2(x[i] + (v_log2 - yref + kQ8Shift));
-                        f[1][i] = ex2(x[i + 2] + (v_log2 - yref + kQ8Shift));
+                        const float ref = m[nt][i] == -INFINITY ? 0.f : m[nt][i];
+                        const float up = v_log2 + kQ8Shift - (my[nt][i] == -INFINITY ? 0.f : my[nt][i]);
+                        l[nt][i] += ex2(s[nt][i] - ref) + ex2(s[nt][i + 2] - ref);
+                        f[0][i] = ex2(s[nt][i] + up);
+                        f[1][i] = ex2(s[nt][i + 2] + up);
                     }
                     pf[nt][0] = movm_t(pack_f16x2(f[0][0], f[0][1]));
                     pf[nt][1] = movm_t(pack_f16x2(f[1][0], f[1][1]));
-#pragma unroll
-                    for (int d = 0; d < 8; ++d) {
-                        o[d][nt][0] *= al[0];
-                        o[d][nt][1] *= al[1];
-                        o[d][nt][2] *= al[0];
-                        o[d][nt][3] *= al[1];
-                    }
                 }
                 // V^T: rows of tile d are dims 16 d + 2 g (first eight) and 16 d + 2 g + 1
 #pragma unroll
                 for (int p = 0; p < 8; p += 2) {
                     uint32_t r[4];
-                    ldsm_x4_t(st + 16 * 128 + mrow * 128 + (((p + mpiece) ^ (mrow & 7)) * 16), r);
+                    ldsm_x4_t(st + 16 * 128 + (((p + mpiece) ^ mx7) << 4), r);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint32_t v0 = __byte_perm(r[2 * i], 0u, 0x3120);
-                        const uint32_t v1 = __byte_perm(r[2 * i + 1], 0u, 0x3120);
-                        const uint32_t a0 = e4m3x2_f16x2(v0), a1 = e4m3x2_f16x2_hi(v0);
-                        const uint32_t a2 = e4m3x2_f16x2(v1), a3 = e4m3x2_f16x2_hi(v1);
+                        uint32_t a0, a1, a2, a3;
+                        e4m3x4_f16(__byte_perm(r[2 * i], 0u, 0x3120), a0, a1);
+                        e4m3x4_f16(__byte_perm(r[2 * i + 1], 0u, 0x3120), a2, a3);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
                             mma_f16(o[p + i][nt], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
@@ -553,12 +615,9 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 x += __shfl_xor_sync(0xffffffffu, x, 4);
                 x += __shfl_xor_sync(0xffffffffu, x, 8);
                 x += __shfl_xor_sync(0xffffffffu, x, 16);
-                if (g == 0) {
-                    float* st = s_stat[warp][8 * nt + 2 * t + i];
-                    st[0] = m[nt][i];
-                    st[1] = my[nt][i];
-                    st[2] = x;
-                }
+                if (g == 0)
+                    *reinterpret_cast<float4*>(s_stat[warp][8 * nt + 2 * t + i]) =
+                        make_float4(m[nt][i], my[nt][i], x, 0.f);
             }
         __syncthreads();  // statistics are there; every warp is done with its ring
         float* s_o = reinterpret_cast<float*>(q8_smem);  // [warp][row][128]
@@ -572,38 +631,43 @@ q8_attn_kernel(const Q8AttnArgs a) {
                                                16 * d + 2 * g) =
                         make_float2(o[d][nt][i], o[d][nt][i + 2]);
         __syncthreads();
-        const bool whole = c0 == 0 && c1 == n;
-        const int slot = c0 > 0 ? 0 : 1;  // the CTA's first segment can only start inside a pair,
-                                          // and only its last can end inside one
-        const int d = threadIdx.x;  // element of the head
-        for (int r = 0; r < 8 * NT; ++r) {
+        const bool whole = c0 == 0 && c1 == (int)n;
+        const int part_slot = c0 > 0 ? 0 : 1;  // the CTA's first segment can only start inside a
+                                               // pair, and only its last can end inside one
+        for (int r = warp; r < 8 * NT; r += 4) {
             const int rr = rb * a.rows + r;
-            if (rr >= a.tokens * a.G) break;
+            if (rr >= total_rows) break;
+            float4 st[4];
             float M = -INFINITY, Y = -INFINITY;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                M = fmaxf(M, s_stat[w][r][0]);
-                Y = fmaxf(Y, s_stat[w][r][1]);
+                st[w] = *reinterpret_cast<const float4*>(s_stat[w][r]);
+                M = fmaxf(M, st[w].x);
+                Y = fmaxf(Y, st[w].y);
             }
-            float L = 0.f, A = 0.f;
+            float L = 0.f;
+            float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                L += s_stat[w][r][2] * q8_weight(s_stat[w][r][0], M);
-                A += s_o[(w * 8 * NT + r) * kHeadDim + d] * q8_weight(s_stat[w][r][1], Y);
+                L += st[w].z * q8_weight(st[w].x, M);
+                const float f = q8_weight(st[w].y, Y);
+                const float4 x = *reinterpret_cast<const float4*>(
+                    s_o + (w * 8 * NT + r) * kHeadDim + 4 * lane);
+                A.x = fmaf(x.x, f, A.x);
+                A.y = fmaf(x.y, f, A.y);
+                A.z = fmaf(x.z, f, A.z);
+                A.w = fmaf(x.w, f, A.w);
             }
             if (whole) {
                 const int tok = rr / a.G, hh = rr - tok * a.G;
-                const float f = Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift);
-                a.out[(((int64_t)b * a.tokens + tok) * a.hq + (int64_t)h * a.G + hh) * kHeadDim + d] =
-                    __float2bfloat16_rn(A / L * f);
+                const float f = (Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift)) / L;
+                *reinterpret_cast<uint2*>(
+                    a.out + (((int64_t)b * a.tokens + tok) * a.hq + (int64_t)h * a.G + hh) * kHeadDim +
+                    4 * lane) = make_uint2(pack_bf16x2(A.x * f, A.y * f), pack_bf16x2(A.z * f, A.w * f));
             } else {
-                float* p = a.part + (((int64_t)blockIdx.x * 2 + slot) * a.rows + r) * kQ8PartFloats;
-                p[d] = A;
-                if (d == 0) {
-                    p[kHeadDim] = M;
-                    p[kHeadDim + 1] = Y;
-                    p[kHeadDim + 2] = L;
-                }
+                float* p = a.part + (((int64_t)blockIdx.x * 2 + part_slot) * a.rows + r) * kQ8PartFloats;
+                *reinterpret_cast<float4*>(p + 4 * lane) = A;
+                if (lane == 0) *reinterpret_cast<float4*>(p + kHeadDim) = make_float4(M, Y, L, 0.f);
             }
         }
         __syncthreads();  // the ring and the statistics may be written again
@@ -611,48 +675,106 @@ q8_attn_kernel(const Q8AttnArgs a) {
     }
 }
 
-// One CTA per (sequence, query row): adds the parts of a pair that several CTAs share, in
-// order of their slots, and writes the zeros of idle sequences.
-__global__ void __launch_bounds__(kHeadDim) q8_merge_kernel(const Q8AttnArgs a) {
-    __shared__ int s_end[NK_Q8_MAX_BATCH];
+// 2^lg_wpr warps per query row: adds the parts of a pair that several CTAs share (each warp its
+// share of the parts in order of their slots, then the warps in order), and writes the zeros
+// of idle sequences. Lane l holds elements 4l .. 4l + 3 of the row.
+__global__ void __launch_bounds__(32 * kQ8MergeWarps) q8_merge_kernel(const Q8AttnArgs a) {
+    __shared__ float4 s_a[kQ8MergeWarps][32], s_st[kQ8MergeWarps];
     if (threadIdx.x == 0) griddep_launch_dependents();
     griddep_wait();
-    q8_units(a, s_end);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int wpr = 1 << a.lg_wpr, sub = warp & (wpr - 1);
     const int b = blockIdx.y;
-    const int row = blockIdx.x;                      // t * hq + head
+    const int row = blockIdx.x * (kQ8MergeWarps >> a.lg_wpr) + (warp >> a.lg_wpr);  // t * hq + head
+    const bool live = row < a.tokens * a.hq;
+    // units of the sequences before b, of b and of all
+    uint32_t before = 0, all = 0;
+#pragma unroll 4
+    for (int i = lane; i < a.batch; i += 32) {
+        const uint32_t x = q8_seq_units(a, i);
+        all += x;
+        before += i < b ? x : 0;
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    all = __reduce_add_sync(0xffffffffu, all);
+    const uint32_t n = q8_seq_units(a, b);
     const int tok = row / a.hq, head = row - tok * a.hq;
     const int h = head / a.G, rr = tok * a.G + head - h * a.G;
     const int rb = rr / a.rows, r = rr - rb * a.rows;
-    const int d = threadIdx.x;
-    const int per_b = a.hkv * a.row_blocks;
-    const int64_t U = (int64_t)s_end[a.batch - 1] * per_b;
-    const int n = s_end[b] - (b > 0 ? s_end[b - 1] : 0);
-    __nv_bfloat16* out = a.out + (((int64_t)b * a.tokens + tok) * a.hq + head) * kHeadDim + d;
+    const uint32_t per_b = a.hkv * a.row_blocks;
+    uint2* out = reinterpret_cast<uint2*>(
+        a.out + (((int64_t)b * a.tokens + tok) * a.hq + head) * kHeadDim + 4 * lane);
     if (n == 0) {
-        *out = __float2bfloat16_rn(0.f);
+        if (live && sub == 0) *out = make_uint2(0u, 0u);
         return;
     }
-    const int G = (int)min((int64_t)a.grid, U);
-    const int64_t p0 = (b > 0 ? (int64_t)s_end[b - 1] * per_b : 0) + (int64_t)(h * a.row_blocks + rb) * n;
-    const int cf = q8_cta_of(U, G, p0), cl = q8_cta_of(U, G, p0 + n - 1);
-    if (cf == cl) return;  // written by that CTA
-    auto part = [&](int c) {  // the first CTA's part starts the pair (slot 1), the others' do not
-        return a.part + (((int64_t)c * 2 + (c == cf ? 1 : 0)) * a.rows + r) * kQ8PartFloats;
-    };
-    float M = -INFINITY, Y = -INFINITY;
-    for (int c = cf; c <= cl; ++c) {
-        const float* p = part(c);
-        M = fmaxf(M, p[kHeadDim]);
-        Y = fmaxf(Y, p[kHeadDim + 1]);
+    const uint32_t U = all * per_b;
+    const Q8Split split(U, min((uint32_t)a.grid, U));
+    const uint32_t p0 = before * per_b + (h * a.row_blocks + rb) * n;
+    const int cf = live ? split.cta_of(p0) : 0, cl = live ? split.cta_of(p0 + n - 1) : 0;
+    const bool shared_pair = cf != cl;  // (else that CTA wrote the row, or there is no row)
+    const int parts = cl - cf + 1;
+    const int i0 = sub * parts >> a.lg_wpr, i1 = (sub + 1) * parts >> a.lg_wpr;
+    float M = -INFINITY, Y = -INFINITY, L = 0.f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (shared_pair) {
+        for (int i = i0; i < i1; i += 4) {  // four parts' loads together
+            float4 x[4], st[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int c = cf + min(i + k, i1 - 1);
+                // the first CTA's part starts the pair (slot 1), the others' do not
+                const float* p = a.part + (((int64_t)c * 2 + (c == cf ? 1 : 0)) * a.rows + r) * kQ8PartFloats;
+                st[k] = *reinterpret_cast<const float4*>(p + kHeadDim);
+                x[k] = *reinterpret_cast<const float4*>(p + 4 * lane);
+            }
+            float Mn = M, Yn = Y;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                Mn = fmaxf(Mn, st[k].x);
+                Yn = fmaxf(Yn, st[k].y);
+            }
+            L *= q8_weight(M, Mn);
+            const float fa = q8_weight(Y, Yn);
+            A.x *= fa; A.y *= fa; A.z *= fa; A.w *= fa;
+            M = Mn;
+            Y = Yn;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (i + k >= i1) break;
+                L += st[k].z * q8_weight(st[k].x, M);
+                const float f = q8_weight(st[k].y, Y);
+                A.x = fmaf(x[k].x, f, A.x);
+                A.y = fmaf(x[k].y, f, A.y);
+                A.z = fmaf(x[k].z, f, A.z);
+                A.w = fmaf(x[k].w, f, A.w);
+            }
+        }
     }
-    float L = 0.f, A = 0.f;
-    for (int c = cf; c <= cl; ++c) {
-        const float* p = part(c);
-        L += p[kHeadDim + 2] * q8_weight(p[kHeadDim], M);
-        A += p[d] * q8_weight(p[kHeadDim + 1], Y);
+    if (wpr > 1) {  // the row's warps, in order
+        s_a[warp][lane] = A;
+        if (lane == 0) s_st[warp] = make_float4(M, Y, L, 0.f);
+        __syncthreads();
+        if (sub != 0) return;
+        for (int w = 0; w < wpr; ++w) {
+            M = fmaxf(M, s_st[warp + w].x);
+            Y = fmaxf(Y, s_st[warp + w].y);
+        }
+        L = 0.f;
+        A = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < wpr; ++w) {
+            const float4 st = s_st[warp + w], x = s_a[warp + w][lane];
+            L += st.z * q8_weight(st.x, M);
+            const float f = q8_weight(st.y, Y);
+            A.x = fmaf(x.x, f, A.x);
+            A.y = fmaf(x.y, f, A.y);
+            A.z = fmaf(x.z, f, A.z);
+            A.w = fmaf(x.w, f, A.w);
+        }
     }
-    const float f = Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift);
-    *out = __float2bfloat16_rn(A / L * f);
+    if (!shared_pair) return;
+    const float f = (Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift)) / L;
+    *out = make_uint2(pack_bf16x2(A.x * f, A.y * f), pack_bf16x2(A.z * f, A.w * f));
 }
 
 static bool q8_heads_ok(int tokens, int hq, int hkv) {
@@ -683,12 +805,18 @@ static int q8_launch_attn(Q8AttnArgs a, cudaStream_t s) {
             return NK_ERR_CUDA;
         slots[dev] = min(sms * per_sm, kQ8MaxGrid);
     }
-    const int64_t most = (int64_t)((a.capacity + kQ8Unit - 1) / kQ8Unit) * a.batch * a.hkv * a.row_blocks;
+    const int64_t pairs = (int64_t)a.batch * a.hkv * a.row_blocks;
+    const int64_t most = (int64_t)((a.capacity + kQ8Unit - 1) / kQ8Unit) * pairs;
     a.grid = (int)min((int64_t)slots[dev], most);
     const int rc = launch_pdl_smem(q8_attn_kernel<NT>, dim3(a.grid), dim3(kQ8AttnThreads),
                                    (size_t)kQ8AttnSmem, s, a);
     if (rc != NK_OK) return rc;
-    return launch_pdl_smem(q8_merge_kernel, dim3(a.tokens * a.hq, a.batch), dim3(kHeadDim), 0, s, a);
+    // about grid / pairs parts to a row: up to eight warps share them, at least two each
+    a.lg_wpr = 0;
+    while (a.lg_wpr < 3 && (int64_t)a.grid > pairs * (4 << a.lg_wpr)) ++a.lg_wpr;
+    const int per_cta = kQ8MergeWarps >> a.lg_wpr;
+    return launch_pdl_smem(q8_merge_kernel, dim3((a.tokens * a.hq + per_cta - 1) / per_cta, a.batch),
+                           dim3(32 * kQ8MergeWarps), 0, s, a);
 }
 
 }  // namespace nk
@@ -773,8 +901,9 @@ extern "C" int nk_attention_decode_q8(const void* q, const void* k_codes, const 
     a.G = q_heads / kv_heads;
     a.rows = q8_rows(tokens * a.G);
     a.row_blocks = (tokens * a.G + a.rows - 1) / a.rows;
-    const int64_t most = (int64_t)((capacity + kQ8Unit - 1) / kQ8Unit) * batch;
-    if (most > (1 << 30)) return NK_ERR_SHAPE;  // running sums of units are 32-bit
+    // units of the whole launch are counted in 32 bits
+    if ((int64_t)((capacity + kQ8Unit - 1) / kQ8Unit) * batch * kv_heads * a.row_blocks > (1 << 30))
+        return NK_ERR_SHAPE;
     if (!ws || ws_bytes < nk_attention_q8_ws_bytes(tokens, q_heads, kv_heads))
         return NK_ERR_WORKSPACE;
     if ((((uintptr_t)q | (uintptr_t)position | (uintptr_t)out) & 7u) ||
@@ -796,7 +925,7 @@ extern "C" int nk_attention_decode_q8(const void* q, const void* k_codes, const 
     a.hq = q_heads;
     a.hkv = kv_heads;
     a.capacity = capacity;
-    a.block = block;
+    a.lg_block = __builtin_ctz(block);
     a.blocks = (capacity + block - 1) / block;
     a.cb = cache_batch_stride;
     a.ch = cache_head_stride;
