@@ -36,20 +36,28 @@ extern "C" {
 #define NK_W4_SCALE_BF16 0
 #define NK_W4_SCALE_FP16 1
 
+/* A weight in this storage. codes, scales and zeros (or NULL) 16-byte aligned. */
+typedef struct nk_w4_weight {
+    const void* codes;
+    const void* scales;
+    const void* zeros;
+    int32_t N, K;
+    int32_t group;       /* 32, 64 or 128                       */
+    int32_t scale_type;  /* NK_W4_SCALE_*                       */
+} nk_w4_weight;
+
 /* Bytes of the three arrays above (0 for arguments out of range: N, K >= 1, group 32, 64 or
  * 128). */
 NK_API size_t nk_w4_code_bytes(int N, int K);
 NK_API size_t nk_w4_scale_bytes(int N, int K, int group);
 NK_API size_t nk_w4_zero_bytes(int N, int K, int group);
 
-/* x: [M, K] bf16, row stride ldx >= K (elements); y: [M, N] bf16, row stride ldy >= N. codes,
- * scales and zeros (or NULL) 16-byte aligned; x and y 2-byte aligned (x 16-byte aligned with
- * ldx % 8 == 0 is read in 16-byte pieces). Any M >= 1. No workspace. The weights must have been
- * written before the launch that precedes this one on the stream (they are read ahead of it);
- * weights made at load time always are. */
-NK_API int nk_gemm_w4(const void* x, int64_t ldx, const void* codes, const void* scales,
-                      const void* zeros, void* y, int64_t ldy, int M, int N, int K, int group,
-                      int scale_type, nk_stream_t stream);
+/* x: [M, K] bf16, row stride ldx >= K (elements); y: [M, N] bf16, row stride ldy >= N; both 2-byte
+ * aligned (x 16-byte aligned with ldx % 8 == 0 is read by TMA). Any M from 1 to 2^20. No
+ * workspace. The weights must have been written before the launch that precedes this one on the
+ * stream (they are read ahead of it); weights made at load time always are. */
+NK_API int nk_gemm_w4(const void* x, int64_t ldx, const nk_w4_weight* w, void* y, int64_t ldy,
+                      int M, nk_stream_t stream);
 
 /* ---- KV cache in 8 bits -------------------------------------------------------------------
  *
@@ -68,42 +76,52 @@ NK_API int nk_gemm_w4(const void* x, int64_t ldx, const void* codes, const void*
 #define NK_Q8_MAX_TOKENS 16
 #define NK_Q8_MAX_BATCH 1024
 
-/* Per-head RMSNorm and RoPE of the new tokens' query and key heads exactly as
- * nk_qk_norm_rope_cache_bf16 rounds them; queries to q_out, keys and values appended to the
- * cache. For each block that the new tokens touch, with amax their largest finite magnitude
+typedef struct nk_q8_cache {
+    void* k_codes;         /* 16-byte aligned                             */
+    void* v_codes;
+    float* k_scale;
+    float* v_scale;
+    int32_t batch;         /* 1..1024                                     */
+    int32_t kv_heads;
+    int32_t head_dim;      /* 128                                         */
+    int32_t capacity;      /* token slots, up to 2^30                     */
+    int32_t block;         /* 16, 32, 64 or 128                           */
+    int32_t reserved;
+    int64_t batch_stride;  /* bytes, multiples of 16                      */
+    int64_t head_stride;
+    int64_t seq_stride;
+} nk_q8_cache;
+
+/* Per-head RMSNorm and RoPE of the new tokens' query and key heads with the cast points of
+ * nk_qk_norm_rope_cache_bf16; queries to q_out, keys and values appended to the cache. For each
+ * block that the new tokens touch, with amax their largest finite magnitude
  * in it: scale = max(former scale if the block holds earlier tokens, smallest power of two
  * s >= 2^-64 with amax <= 448 s, 0 for amax = 0). When the scale rises, the earlier tokens' codes c
  * become e4m3_rne(c * former / new); new codes are e4m3_rne(value / scale), NaN for a value
- * that is not finite. Slots past the new tokens, and everything of an idle sequence (its q_out rows included), are
- * left as they are.
+ * that is not finite. Slots past the new tokens, and everything of an idle sequence (its q_out
+ * rows included), are left as they are.
  *   qkv: [batch * tokens, (q_heads + 2 kv_heads) * 128] bf16, row stride ld_qkv, row b * tokens + t
  *   q_out: [batch * tokens, q_heads * 128] bf16; q_norm, k_norm: [128]; cos, sin: [capacity, 128]
  * bf16 pointers 8-byte aligned and ld_qkv a multiple of 4. */
 NK_API int nk_qk_norm_rope_cache_q8(const void* qkv, int64_t ld_qkv, const void* q_norm,
                                     const void* k_norm, const void* cos_table,
                                     const void* sin_table, const int64_t* position,
-                                    int per_sequence, void* q_out, void* k_codes, void* v_codes,
-                                    float* k_scale, float* v_scale, int batch, int tokens,
-                                    int q_heads, int kv_heads, int head_dim, int capacity,
-                                    int block, int64_t cache_batch_stride,
-                                    int64_t cache_head_stride, int64_t cache_seq_stride,
-                                    float eps, nk_stream_t stream);
+                                    int per_sequence, void* q_out, const nk_q8_cache* cache,
+                                    int tokens, int q_heads, float eps, nk_stream_t stream);
 
 /* Workspace bytes of nk_attention_decode_q8, whatever the batch and capacity (0: out of range).
- * It needs no initialisation; calls that share one must be ordered. */
+ * It needs no initialisation. One workspace serves any sequence of ordered calls with up to as
+ * many tokens; calls that may overlap on the GPU (streams, graphs) need one each. */
 NK_API size_t nk_attention_q8_ws_bytes(int tokens, int q_heads, int kv_heads);
 
 /* Grouped attention of the new tokens over the cache: query row (b, t, h) sees slots
  * 0 .. position + t of kv head h / (q_heads / kv_heads); fp32 scores, softmax and sums, rounded
  * once to bf16; rows of idle sequences are zero. q, out: [batch * tokens, q_heads * 128] bf16,
- * 8-byte aligned. q_heads / kv_heads between 1 and 16; batch <= 1024. */
-NK_API int nk_attention_decode_q8(const void* q, const void* k_codes, const void* v_codes,
-                                  const float* k_scale, const float* v_scale,
-                                  const int64_t* position, int per_sequence, void* out, int batch,
-                                  int tokens, int q_heads, int kv_heads, int head_dim,
-                                  int capacity, int block, int64_t cache_batch_stride,
-                                  int64_t cache_head_stride, int64_t cache_seq_stride,
-                                  float scale, void* ws, size_t ws_bytes, nk_stream_t stream);
+ * 8-byte aligned. q_heads / kv_heads between 1 and 16; ws 16-byte aligned. */
+NK_API int nk_attention_decode_q8(const void* q, const nk_q8_cache* cache,
+                                  const int64_t* position, int per_sequence, void* out, int tokens,
+                                  int q_heads, float scale, void* ws, size_t ws_bytes,
+                                  nk_stream_t stream);
 
 #ifdef __cplusplus
 }

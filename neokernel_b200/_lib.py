@@ -82,6 +82,24 @@ class NkPlan(ctypes.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class NkW4Weight(ctypes.Structure):
+    """``nk_w4_weight`` (include/nk_quant.h)."""
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("zeros", ctypes.c_void_p), ("N", ctypes.c_int32), ("K", ctypes.c_int32),
+                ("group", ctypes.c_int32), ("scale_type", ctypes.c_int32)]
+
+
+class NkQ8Cache(ctypes.Structure):
+    """``nk_q8_cache`` (include/nk_quant.h)."""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("batch", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("capacity", ctypes.c_int32),
+                ("block", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("batch_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("seq_stride", ctypes.c_int64)]
+
+
 class NkError(RuntimeError):
     """A non-zero status from libnkgemm.so."""
 
@@ -167,16 +185,16 @@ def load() -> ctypes.CDLL:
     L.nk_w4_scale_bytes.restype = ctypes.c_size_t
     L.nk_w4_zero_bytes.argtypes = [i32, i32, i32]
     L.nk_w4_zero_bytes.restype = ctypes.c_size_t
-    L.nk_gemm_w4.argtypes = [vp, i64, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, vp]
+    # the descriptors (nk_w4_weight, nk_q8_cache) go by address: one conversion a call
+    L.nk_gemm_w4.argtypes = [vp, i64, vp, vp, i64, i32, vp]
     L.nk_gemm_w4.restype = i32
-    L.nk_qk_norm_rope_cache_q8.argtypes = [vp, i64, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp,
-                                           i32, i32, i32, i32, i32, i32, i32, i64, i64, i64, f32,
+    L.nk_qk_norm_rope_cache_q8.argtypes = [vp, i64, vp, vp, vp, vp, vp, i32, vp, vp, i32, i32, f32,
                                            vp]
     L.nk_qk_norm_rope_cache_q8.restype = i32
     L.nk_attention_q8_ws_bytes.argtypes = [i32, i32, i32]
     L.nk_attention_q8_ws_bytes.restype = ctypes.c_size_t
-    L.nk_attention_decode_q8.argtypes = [vp, vp, vp, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32,
-                                         i32, i32, i64, i64, i64, f32, vp, ctypes.c_size_t, vp]
+    L.nk_attention_decode_q8.argtypes = [vp, vp, vp, i32, vp, i32, i32, f32, vp, ctypes.c_size_t,
+                                         vp]
     L.nk_attention_decode_q8.restype = i32
     L.nk_device_error.argtypes = [vp, ctypes.POINTER(i32)]
     L.nk_device_error.restype = i32

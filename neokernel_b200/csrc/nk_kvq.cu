@@ -235,14 +235,24 @@ __global__ void __launch_bounds__(32 * kQ8Warps) q8_append_kernel(const Q8Append
 // term), while the sum l = sum 2^(x - m) stays in fp32. Then out = (O / l) 2^(my - m).
 //
 // A pair covered by one CTA is written directly; otherwise its CTAs write (m, my, l, O) of their
-// part, and a second launch adds the parts in order of their slots.
+// part, and a second launch adds the parts in order of their slots, its rows spread over the
+// GPU. (Measured: the last CTA of a pair adding the parts in the first launch instead takes
+// 11.2 us where the two launches take 8.5, at one sequence of 1024 slots, and 60 where they take
+// 30 at five of 3000 with 32 query rows: one CTA walks through all rows of the pair.)
 // ---------------------------------------------------------------------------------------
 constexpr int kQ8Unit = 64;                 // slots per unit, 16 per warp
 constexpr int kQ8AttnThreads = 128;
-constexpr int kQ8Stages = 4;                // units in flight per warp
+constexpr int kQ8Stages = 2;                // units in flight per warp (with four, an SM has no room for
+                                            // the next launch's CTAs: 2 x 128k slots 86 -> 101 us)
 constexpr int kQ8WarpStage = 2 * 16 * 128;  // K and V rows of 16 slots
-constexpr int kQ8Ring = kQ8Stages * 4 * kQ8WarpStage;         // 64 KB
-constexpr int kQ8AttnSmem = kQ8Ring + 4 * kQ8Stages * 8;      // and each stage's two scales
+constexpr int kQ8Ring = kQ8Stages * 4 * kQ8WarpStage;         // 32 KB
+constexpr int kQ8OPitch = kHeadDim + 4;      // floats; spreads a warp's rows over the banks
+__host__ __device__ constexpr int q8_o_bytes(int nt) { return 4 * 8 * nt * kQ8OPitch * 4; }
+// the ring (or, once it is idle, the warps' sums), then each stage's two scales
+__host__ __device__ constexpr int q8_scale_off(int nt) {
+    return kQ8Ring > q8_o_bytes(nt) ? kQ8Ring : q8_o_bytes(nt);
+}
+__host__ __device__ constexpr int q8_attn_smem(int nt) { return q8_scale_off(nt) + 4 * kQ8Stages * 8; }
 constexpr int kQ8MaxGrid = 148 * 4;
 constexpr int kQ8PartFloats = kHeadDim + 4; // O, then m, my, l
 constexpr float kQ8Shift = 15.f;            // probabilities are held times 2^15
@@ -255,8 +265,8 @@ struct Q8AttnArgs {
     const int64_t* position; int per_sequence;
     __nv_bfloat16* out;
     float* part;                 // [grid][2][rows][kQ8PartFloats]
-    int batch, tokens, hq, hkv, G, capacity, lg_block, blocks;
-    int rows, row_blocks;        // query rows of a CTA (8 NT), row blocks of T * G rows
+    int batch, tokens, hq, hkv, G, g_mul, capacity, lg_block, blocks;
+    int rows, row_blocks;        // query rows of a CTA (8 NT), row blocks of a pair's T * G rows
     int grid;                    // CTAs of the first launch
     int lg_wpr;                  // merge: log2 of the warps that share a row
     int64_t cb, ch, cs;
@@ -331,12 +341,13 @@ struct Q8Split {
 };
 
 template <int NT>
-__global__ void __launch_bounds__(kQ8AttnThreads, NT <= 2 ? 3 : 2)
+__global__ void __launch_bounds__(kQ8AttnThreads, 3)
 q8_attn_kernel(const Q8AttnArgs a) {
     extern __shared__ __align__(1024) uint8_t q8_smem[];
     __shared__ int s_end[NK_Q8_MAX_BATCH];              // running sum of the sequences' units
     __shared__ float s_stat[4][8 * NT][4];
     __shared__ uint2 s_q[NT > 1 ? NT * 8 * 32 : 1];     // Q^T operand, shared by the warps
+    __shared__ float s_down[8 * NT];                    // and its rows' powers of two
     if (threadIdx.x == 0) griddep_launch_dependents();
     griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -373,13 +384,21 @@ q8_attn_kernel(const Q8AttnArgs a) {
     const uint32_t per_b = a.hkv * a.row_blocks;            // pairs per sequence
     const uint32_t U = s_end[a.batch - 1] * per_b;
     const uint32_t G = min((uint32_t)a.grid, U);            // no CTA of the partition is empty
+    const int total_rows = a.tokens * a.G;
+    // rows of idle sequences are zero
+    for (int b = blockIdx.x; b < a.batch; b += a.grid)
+        if (s_end[b] == (b > 0 ? s_end[b - 1] : 0)) {
+            const int vecs = a.tokens * a.hq * (kHeadDim / 4);
+            uint2* o = reinterpret_cast<uint2*>(a.out + (int64_t)b * a.tokens * a.hq * kHeadDim);
+            for (int i = threadIdx.x; i < vecs; i += kQ8AttnThreads) o[i] = make_uint2(0u, 0u);
+        }
     if (blockIdx.x >= G) return;
     const Q8Split split(U, G);
     uint32_t u = split.begin(blockIdx.x);
     const uint32_t u_end = split.begin(blockIdx.x + 1);
     const uint32_t smem0 = static_cast<uint32_t>(__cvta_generic_to_shared(q8_smem));
     const uint32_t ring = smem0 + warp * (kQ8Stages * kQ8WarpStage);
-    const uint32_t s_scale = smem0 + kQ8Ring + warp * (kQ8Stages * 8);
+    const uint32_t s_scale = smem0 + q8_scale_off(NT) + warp * (kQ8Stages * 8);
 
     while (u < u_end) {
         // the pair of unit u: sequence b, kv head h, row block rb; its units [p0, p0 + n)
@@ -411,14 +430,23 @@ q8_attn_kernel(const Q8AttnArgs a) {
             if (fill < c1) {
                 const uint32_t st = fill & (kQ8Stages - 1);
                 const uint32_t dst = ring + st * kQ8WarpStage;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool ok = slot + 4 * i < len;
-                    const uint32_t d = dst + (i & 1 ? d1 : d0) + i * 512;
-                    cp_async<16>(d, ok ? kp + i * row4 : a.k, ok);
-                    cp_async<16>(d + 16 * 128, ok ? vp + i * row4 : a.v, ok);
-                }
                 const int s0 = fill * kQ8Unit + warp * 16;
+                if (s0 + 16 <= len) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t d = dst + (i & 1 ? d1 : d0) + i * 512;
+                        cp_async<16>(d, kp + i * row4, true);
+                        cp_async<16>(d + 16 * 128, vp + i * row4, true);
+                    }
+                } else {  // the sequence ends in this tile: what is past it reads as zero
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool ok = slot + 4 * i < len;
+                        const uint32_t d = dst + (i & 1 ? d1 : d0) + i * 512;
+                        cp_async<16>(d, ok ? kp + i * row4 : a.k, ok);
+                        cp_async<16>(d + 16 * 128, ok ? vp + i * row4 : a.v, ok);
+                    }
+                }
                 if (lane < 2 && s0 < len)
                     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(
                                      s_scale + st * 8 + lane * 4), "l"(sp + (s0 >> a.lg_block))
@@ -433,16 +461,17 @@ q8_attn_kernel(const Q8AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < kQ8Stages - 1; ++i) issue();
 
-        // Q^T operand: column g of tile nt is query row 8 nt + g; dims 16 s + 4 t .. + 3 of step s
+        // Q^T operand: column g of tile nt is query row 8 nt + g; dims 16 s + 4 t .. + 3 of step s.
+        // With several tiles the warps take turns and share them through shared memory.
         uint2 qf[NT > 1 ? 1 : 8];
         float qs[NT][2];     // 2^-shift of rows 8 nt + 2t, + 1, times the softmax scale
         int last[NT][2];     // last slot those rows see, relative to pos (-1: no such row)
-        const int total_rows = a.tokens * a.G;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            if (NT > 1 && warp % NT != nt) continue;
             const int r = rb * a.rows + 8 * nt + g;
             const bool ok = r < total_rows;
-            const int tok = ok ? r / a.G : 0, hh = ok ? r - tok * a.G : 0;
+            const int tok = ok ? r * a.g_mul >> 16 : 0, hh = ok ? r - tok * a.G : 0;
             const __nv_bfloat16* src =
                 a.q + (((int64_t)b * a.tokens + tok) * a.hq + (int64_t)h * a.G + hh) * kHeadDim + 4 * t;
             uint2 w[8];
@@ -465,23 +494,34 @@ q8_attn_kernel(const Q8AttnArgs a) {
             for (int s = 0; s < 8; ++s) {
                 const uint2 f = make_uint2(pack_f16x2(bf16lo(w[s].x) * up, bf16hi(w[s].x) * up),
                                            pack_f16x2(bf16lo(w[s].y) * up, bf16hi(w[s].y) * up));
-                if (NT == 1) qf[s] = f;
-                else if ((nt & 3) == warp % NT || NT == 1) s_q[(nt * 8 + s) * 32 + lane] = f;
+                if (NT == 1) qf[NT == 1 ? s : 0] = f;
+                else s_q[(nt * 8 + s) * 32 + lane] = f;
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                qs[nt][i] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + i)) * a.scale_log2;
-                const int rr = rb * a.rows + 8 * nt + 2 * t + i;
-                last[nt][i] = rr < total_rows ? rr / a.G : -1;
+            if (NT == 1) {
+                qs[0][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+                qs[0][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+            } else if (t == 0) {
+                s_down[8 * nt + g] = down;
             }
         }
         if (NT > 1) __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                qs[nt][i] = (NT == 1 ? qs[nt][i] : s_down[8 * nt + 2 * t + i]) * a.scale_log2;
+                const int rr = rb * a.rows + 8 * nt + 2 * t + i;
+                last[nt][i] = rr < total_rows ? rr * a.g_mul >> 16 : -1;
+            }
 
-        float m[NT][2], my[NT][2], l[NT][2], o[8][NT][4];
+        // m, my: running maxima of x and x + log2 s_v; ref, off: what the exponents subtract (0 while
+        // nothing was seen)
+        float m[NT][2], my[NT][2], ref[NT][2], off[NT][2], l[NT][2], o[8][NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             m[nt][0] = m[nt][1] = my[nt][0] = my[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.f;
+            ref[nt][0] = ref[nt][1] = l[nt][0] = l[nt][1] = 0.f;
+            off[nt][0] = off[nt][1] = kQ8Shift;
 #pragma unroll
             for (int d = 0; d < 8; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
         }
@@ -495,7 +535,7 @@ q8_attn_kernel(const Q8AttnArgs a) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kQ8Stages - 1) : "memory");
             __syncwarp();
             const uint32_t stage = c & (kQ8Stages - 1), st = mbase + stage * kQ8WarpStage;
-            const int j0 = c * kQ8Unit + warp * 16;
+            const int j0 = c * kQ8Unit + warp * 16;     // the warp's first slot of the unit
             if (j0 < len) {
                 float k_scale, v_scale;
                 asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(k_scale), "=f"(v_scale)
@@ -509,44 +549,39 @@ q8_attn_kernel(const Q8AttnArgs a) {
                     uint32_t r[4];
                     ldsm_x4(st + (((p + mpiece) ^ mx7) << 4), r);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
+                    for (int k = 0; k < 2; ++k) {
                         uint32_t a0, a1, a2, a3;
-                        e4m3x4_f16(r[2 * i], a0, a2);
-                        e4m3x4_f16(r[2 * i + 1], a1, a3);
+                        e4m3x4_f16(r[2 * k], a0, a2);
+                        e4m3x4_f16(r[2 * k + 1], a1, a3);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            const uint2 f = NT == 1 ? qf[NT == 1 ? p + i : 0]
-                                                    : s_q[(nt * 8 + p + i) * 32 + lane];
+                            const uint2 f = NT == 1 ? qf[NT == 1 ? p + k : 0]
+                                                    : s_q[(nt * 8 + p + k) * 32 + lane];
                             mma_f16(s[nt], a0, a1, a2, a3, f.x, f.y);
                         }
                     }
                 }
-                // scores of slots j0 + g, j0 + 8 + g against rows 2t, 2t + 1 of each tile
-                const int rel = j0 - pos + g;           // slots are seen up to pos + last
-                const bool all_seen = j0 + 15 <= pos;   // by every row
-                float mx[NT][2];
+                // scores of slots j0 + g and j0 + 8 + g against rows 2t, 2t + 1
+                const bool all_seen = j0 + 15 <= pos;
                 bool grown = false;
+                float mx[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float f = qs[nt][i] * k_scale;
-                        s[nt][i] *= f;
-                        s[nt][i + 2] *= f;
-                    }
+                    for (int e = 0; e < 4; ++e) s[nt][e] *= qs[nt][e & 1] * k_scale;
                     if (!all_seen) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (rel + (i >> 1) * 8 > last[nt][i & 1]) s[nt][i] = -INFINITY;
+                        for (int e = 0; e < 4; ++e)
+                            if (j0 - pos + g + (e >> 1) * 8 > last[nt][e & 1]) s[nt][e] = -INFINITY;
                     }
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        float x = fmaxf(s[nt][i], s[nt][i + 2]);
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        mx[nt][i] = x;
-                        grown |= x > m[nt][i] || x + v_log2 > my[nt][i];
+                    for (int e = 0; e < 2; ++e) {
+                        float y = fmaxf(s[nt][e], s[nt][e + 2]);
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+                        mx[nt][e] = y;
+                        grown |= y > m[nt][e] || y + v_log2 > my[nt][e];
                     }
                 }
                 if (__any_sync(0xffffffffu, grown)) {  // a new maximum: rescale the sums
@@ -554,13 +589,16 @@ q8_attn_kernel(const Q8AttnArgs a) {
                     for (int nt = 0; nt < NT; ++nt) {
                         float al[2];
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float mn = fmaxf(m[nt][i], mx[nt][i]);
-                            const float yn = fmaxf(my[nt][i], mx[nt][i] + v_log2);
-                            l[nt][i] *= ex2(m[nt][i] - (mn == -INFINITY ? 0.f : mn));
-                            al[i] = ex2(my[nt][i] - (yn == -INFINITY ? 0.f : yn));
-                            m[nt][i] = mn;
-                            my[nt][i] = yn;
+                        for (int e = 0; e < 2; ++e) {
+                            const float mn = fmaxf(m[nt][e], mx[nt][e]);
+                            const float yn = fmaxf(my[nt][e], mx[nt][e] + v_log2);
+                            ref[nt][e] = mn == -INFINITY ? 0.f : mn;
+                            const float yref = yn == -INFINITY ? 0.f : yn;
+                            l[nt][e] *= ex2(m[nt][e] - ref[nt][e]);
+                            al[e] = ex2(my[nt][e] - yref);
+                            off[nt][e] = kQ8Shift - yref;
+                            m[nt][e] = mn;
+                            my[nt][e] = yn;
                         }
 #pragma unroll
                         for (int d = 0; d < 8; ++d) {
@@ -576,12 +614,12 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 for (int nt = 0; nt < NT; ++nt) {
                     float f[2][2];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float ref = m[nt][i] == -INFINITY ? 0.f : m[nt][i];
-                        const float up = v_log2 + kQ8Shift - (my[nt][i] == -INFINITY ? 0.f : my[nt][i]);
-                        l[nt][i] += ex2(s[nt][i] - ref) + ex2(s[nt][i + 2] - ref);
-                        f[0][i] = ex2(s[nt][i] + up);
-                        f[1][i] = ex2(s[nt][i + 2] + up);
+                    for (int e = 0; e < 2; ++e) {
+                        const float x0 = s[nt][e], x1 = s[nt][e + 2];
+                        const float up = v_log2 + off[nt][e];
+                        l[nt][e] += ex2(x0 - ref[nt][e]) + ex2(x1 - ref[nt][e]);
+                        f[0][e] = ex2(x0 + up);
+                        f[1][e] = ex2(x1 + up);
                     }
                     pf[nt][0] = movm_t(pack_f16x2(f[0][0], f[0][1]));
                     pf[nt][1] = movm_t(pack_f16x2(f[1][0], f[1][1]));
@@ -592,13 +630,13 @@ q8_attn_kernel(const Q8AttnArgs a) {
                     uint32_t r[4];
                     ldsm_x4_t(st + 16 * 128 + (((p + mpiece) ^ mx7) << 4), r);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
+                    for (int k = 0; k < 2; ++k) {
                         uint32_t a0, a1, a2, a3;
-                        e4m3x4_f16(__byte_perm(r[2 * i], 0u, 0x3120), a0, a1);
-                        e4m3x4_f16(__byte_perm(r[2 * i + 1], 0u, 0x3120), a2, a3);
+                        e4m3x4_f16(__byte_perm(r[2 * k], 0u, 0x3120), a0, a1);
+                        e4m3x4_f16(__byte_perm(r[2 * k + 1], 0u, 0x3120), a2, a3);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
-                            mma_f16(o[p + i][nt], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
+                            mma_f16(o[p + k][nt], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
                     }
                 }
             }
@@ -627,16 +665,16 @@ q8_attn_kernel(const Q8AttnArgs a) {
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int d = 0; d < 8; ++d)
-                    *reinterpret_cast<float2*>(s_o + (warp * 8 * NT + 8 * nt + 2 * t + i) * kHeadDim +
+                    *reinterpret_cast<float2*>(s_o + (warp * 8 * NT + 8 * nt + 2 * t + i) * kQ8OPitch +
                                                16 * d + 2 * g) =
                         make_float2(o[d][nt][i], o[d][nt][i + 2]);
         __syncthreads();
         const bool whole = c0 == 0 && c1 == (int)n;
-        const int part_slot = c0 > 0 ? 0 : 1;  // the CTA's first segment can only start inside a
-                                               // pair, and only its last can end inside one
-        for (int r = warp; r < 8 * NT; r += 4) {
-            const int rr = rb * a.rows + r;
-            if (rr >= total_rows) break;
+        // the CTA's first segment can only start inside a pair (slot 0), and only its last can end
+        // inside one that it starts (slot 1)
+        float* part = a.part + ((int64_t)blockIdx.x * 2 + (c0 > 0 ? 0 : 1)) * a.rows * kQ8PartFloats;
+        const int rows = min(8 * NT, total_rows - rb * a.rows);
+        for (int r = warp; r < rows; r += 4) {
             float4 st[4];
             float M = -INFINITY, Y = -INFINITY;
 #pragma unroll
@@ -652,20 +690,20 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 L += st[w].z * q8_weight(st[w].x, M);
                 const float f = q8_weight(st[w].y, Y);
                 const float4 x = *reinterpret_cast<const float4*>(
-                    s_o + (w * 8 * NT + r) * kHeadDim + 4 * lane);
+                    s_o + (w * 8 * NT + r) * kQ8OPitch + 4 * lane);
                 A.x = fmaf(x.x, f, A.x);
                 A.y = fmaf(x.y, f, A.y);
                 A.z = fmaf(x.z, f, A.z);
                 A.w = fmaf(x.w, f, A.w);
             }
             if (whole) {
-                const int tok = rr / a.G, hh = rr - tok * a.G;
+                const int rr = rb * a.rows + r, tok = rr * a.g_mul >> 16, hh = rr - tok * a.G;
                 const float f = (Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift)) / L;
                 *reinterpret_cast<uint2*>(
                     a.out + (((int64_t)b * a.tokens + tok) * a.hq + (int64_t)h * a.G + hh) * kHeadDim +
                     4 * lane) = make_uint2(pack_bf16x2(A.x * f, A.y * f), pack_bf16x2(A.z * f, A.w * f));
             } else {
-                float* p = a.part + (((int64_t)blockIdx.x * 2 + part_slot) * a.rows + r) * kQ8PartFloats;
+                float* p = part + r * kQ8PartFloats;
                 *reinterpret_cast<float4*>(p + 4 * lane) = A;
                 if (lane == 0) *reinterpret_cast<float4*>(p + kHeadDim) = make_float4(M, Y, L, 0.f);
             }
@@ -676,8 +714,7 @@ q8_attn_kernel(const Q8AttnArgs a) {
 }
 
 // 2^lg_wpr warps per query row: adds the parts of a pair that several CTAs share (each warp its
-// share of the parts in order of their slots, then the warps in order), and writes the zeros
-// of idle sequences. Lane l holds elements 4l .. 4l + 3 of the row.
+// share of the parts in order of their slots, then the warps in order). Lane l holds elements 4l .. 4l + 3 of the row.
 __global__ void __launch_bounds__(32 * kQ8MergeWarps) q8_merge_kernel(const Q8AttnArgs a) {
     __shared__ float4 s_a[kQ8MergeWarps][32], s_st[kQ8MergeWarps];
     if (threadIdx.x == 0) griddep_launch_dependents();
@@ -704,10 +741,7 @@ __global__ void __launch_bounds__(32 * kQ8MergeWarps) q8_merge_kernel(const Q8At
     const uint32_t per_b = a.hkv * a.row_blocks;
     uint2* out = reinterpret_cast<uint2*>(
         a.out + (((int64_t)b * a.tokens + tok) * a.hq + head) * kHeadDim + 4 * lane);
-    if (n == 0) {
-        if (live && sub == 0) *out = make_uint2(0u, 0u);
-        return;
-    }
+    if (n == 0) return;  // idle: the first launch wrote the zeros
     const uint32_t U = all * per_b;
     const Q8Split split(U, min((uint32_t)a.grid, U));
     const uint32_t p0 = before * per_b + (h * a.row_blocks + rb) * n;
@@ -784,8 +818,10 @@ static bool q8_heads_ok(int tokens, int hq, int hkv) {
 static bool q8_block_ok(int block) {
     return block == 16 || block == 32 || block == 64 || block == 128;
 }
-// Query rows of one CTA: column tiles of eight, 1, 2 or 4 of them.
-static int q8_rows(int rows) { return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32); }
+// Query rows of one CTA: one or two column tiles of eight. More rows take several CTAs, which read
+// the cache again (from L2): measured against four tiles a CTA, 19.8 us against 22.4 (five
+// sequences of 3000 slots, 32 rows), 185 against 177 (16 of 8192, 64 rows).
+static int q8_rows(int rows) { return rows <= 8 ? 8 : 16; }
 
 template <int NT>
 static int q8_launch_attn(Q8AttnArgs a, cudaStream_t s) {
@@ -796,10 +832,12 @@ static int q8_launch_attn(Q8AttnArgs a, cudaStream_t s) {
     if (slots[dev] == 0) {
         int sms = 0, per_sm = 0;
         if (cudaFuncSetAttribute(q8_attn_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 kQ8AttnSmem) != cudaSuccess ||
+                                 q8_attn_smem(NT)) != cudaSuccess ||
+            cudaFuncSetAttribute(q8_attn_kernel<NT>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 (int)cudaSharedmemCarveoutMaxShared) != cudaSuccess ||
             cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
             cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, q8_attn_kernel<NT>,
-                                                          kQ8AttnThreads, kQ8AttnSmem) !=
+                                                          kQ8AttnThreads, q8_attn_smem(NT)) !=
                 cudaSuccess ||
             per_sm < 1)
             return NK_ERR_CUDA;
@@ -809,7 +847,7 @@ static int q8_launch_attn(Q8AttnArgs a, cudaStream_t s) {
     const int64_t most = (int64_t)((a.capacity + kQ8Unit - 1) / kQ8Unit) * pairs;
     a.grid = (int)min((int64_t)slots[dev], most);
     const int rc = launch_pdl_smem(q8_attn_kernel<NT>, dim3(a.grid), dim3(kQ8AttnThreads),
-                                   (size_t)kQ8AttnSmem, s, a);
+                                   (size_t)q8_attn_smem(NT), s, a);
     if (rc != NK_OK) return rc;
     // about grid / pairs parts to a row: up to eight warps share them, at least two each
     a.lg_wpr = 0;
@@ -819,31 +857,35 @@ static int q8_launch_attn(Q8AttnArgs a, cudaStream_t s) {
                            dim3(32 * kQ8MergeWarps), 0, s, a);
 }
 
+static bool q8_cache_ok(const nk_q8_cache* c, int tokens, int q_heads) {
+    return c->head_dim == kHeadDim && c->batch >= 1 && c->batch <= NK_Q8_MAX_BATCH &&
+           q8_heads_ok(tokens, q_heads, c->kv_heads) && c->capacity >= 1 &&
+           c->capacity <= kQ8MaxCapacity && tokens <= c->capacity && q8_block_ok(c->block) &&
+           c->seq_stride >= c->head_dim;
+}
+static bool q8_cache_aligned(const nk_q8_cache* c) {
+    return !((((uintptr_t)c->k_codes | (uintptr_t)c->v_codes) & 15u) ||
+             (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3u) || c->batch_stride % 16 ||
+             c->head_stride % 16 || c->seq_stride % 16);
+}
+
 }  // namespace nk
 
 extern "C" int nk_qk_norm_rope_cache_q8(const void* qkv, int64_t ld_qkv, const void* q_norm,
                                         const void* k_norm, const void* cos_table,
                                         const void* sin_table, const int64_t* position,
-                                        int per_sequence, void* q_out, void* k_codes,
-                                        void* v_codes, float* k_scale, float* v_scale, int batch,
-                                        int tokens, int q_heads, int kv_heads, int head_dim,
-                                        int capacity, int block, int64_t cache_batch_stride,
-                                        int64_t cache_head_stride, int64_t cache_seq_stride,
-                                        float eps, nk_stream_t stream) {
+                                        int per_sequence, void* q_out, const nk_q8_cache* c,
+                                        int tokens, int q_heads, float eps, nk_stream_t stream) {
     using namespace nk;
-    if (!qkv || !q_norm || !k_norm || !cos_table || !sin_table || !position || !q_out ||
-        !k_codes || !v_codes || !k_scale || !v_scale)
+    if (!qkv || !q_norm || !k_norm || !cos_table || !sin_table || !position || !q_out || !c ||
+        !c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale)
         return NK_ERR_ARG;
-    if (head_dim != kHeadDim || batch < 1 || batch > NK_Q8_MAX_BATCH ||
-        !q8_heads_ok(tokens, q_heads, kv_heads) || capacity < 1 || capacity > kQ8MaxCapacity || tokens > capacity ||
-        !q8_block_ok(block) || ld_qkv < (int64_t)(q_heads + 2 * kv_heads) * head_dim ||
-        cache_seq_stride < head_dim)
+    if (!q8_cache_ok(c, tokens, q_heads) ||
+        ld_qkv < (int64_t)(q_heads + 2 * c->kv_heads) * kHeadDim)
         return NK_ERR_SHAPE;
     if ((((uintptr_t)qkv | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)cos_table |
           (uintptr_t)sin_table | (uintptr_t)position | (uintptr_t)q_out) & 7u) ||
-        (((uintptr_t)k_codes | (uintptr_t)v_codes) & 15u) ||
-        (((uintptr_t)k_scale | (uintptr_t)v_scale) & 3u) || ld_qkv % 4 ||
-        cache_batch_stride % 16 || cache_head_stride % 16 || cache_seq_stride % 16)
+        ld_qkv % 4 || !q8_cache_aligned(c))
         return NK_ERR_ALIGN;
     Q8AppendArgs a{};
     a.qkv = static_cast<const __nv_bfloat16*>(qkv);
@@ -855,24 +897,24 @@ extern "C" int nk_qk_norm_rope_cache_q8(const void* qkv, int64_t ld_qkv, const v
     a.position = position;
     a.per_sequence = per_sequence != 0;
     a.q_out = static_cast<__nv_bfloat16*>(q_out);
-    a.k = static_cast<uint8_t*>(k_codes);
-    a.v = static_cast<uint8_t*>(v_codes);
-    a.ks = k_scale;
-    a.vs = v_scale;
-    a.batch = batch;
+    a.k = static_cast<uint8_t*>(c->k_codes);
+    a.v = static_cast<uint8_t*>(c->v_codes);
+    a.ks = c->k_scale;
+    a.vs = c->v_scale;
+    a.batch = c->batch;
     a.tokens = tokens;
     a.hq = q_heads;
-    a.hkv = kv_heads;
-    a.capacity = capacity;
-    a.block = block;
-    a.blocks = (capacity + block - 1) / block;
-    a.cb = cache_batch_stride;
-    a.ch = cache_head_stride;
-    a.cs = cache_seq_stride;
+    a.hkv = c->kv_heads;
+    a.capacity = c->capacity;
+    a.block = c->block;
+    a.blocks = (c->capacity + c->block - 1) / c->block;
+    a.cb = c->batch_stride;
+    a.ch = c->head_stride;
+    a.cs = c->seq_stride;
     a.eps = eps;
     a.q_ctas = (tokens * q_heads + kQ8Warps - 1) / kQ8Warps;
-    const int touched = (tokens + block - 2) / block + 1;  // blocks that T tokens can touch
-    return launch_pdl_smem(q8_append_kernel, dim3(a.q_ctas + kv_heads * touched, batch),
+    const int touched = (tokens + c->block - 2) / c->block + 1;  // blocks that T tokens can touch
+    return launch_pdl_smem(q8_append_kernel, dim3(a.q_ctas + c->kv_heads * touched, c->batch),
                            dim3(32 * kQ8Warps), 0, (cudaStream_t)stream, a);
 }
 
@@ -883,58 +925,51 @@ extern "C" size_t nk_attention_q8_ws_bytes(int tokens, int q_heads, int kv_heads
            sizeof(float);
 }
 
-extern "C" int nk_attention_decode_q8(const void* q, const void* k_codes, const void* v_codes,
-                                      const float* k_scale, const float* v_scale,
+extern "C" int nk_attention_decode_q8(const void* q, const nk_q8_cache* c,
                                       const int64_t* position, int per_sequence, void* out,
-                                      int batch, int tokens, int q_heads, int kv_heads,
-                                      int head_dim, int capacity, int block,
-                                      int64_t cache_batch_stride, int64_t cache_head_stride,
-                                      int64_t cache_seq_stride, float scale, void* ws,
+                                      int tokens, int q_heads, float scale, void* ws,
                                       size_t ws_bytes, nk_stream_t stream) {
     using namespace nk;
-    if (!q || !k_codes || !v_codes || !k_scale || !v_scale || !position || !out) return NK_ERR_ARG;
-    if (head_dim != kHeadDim || batch < 1 || batch > NK_Q8_MAX_BATCH ||
-        !q8_heads_ok(tokens, q_heads, kv_heads) || capacity < 1 || capacity > kQ8MaxCapacity || tokens > capacity ||
-        !q8_block_ok(block) || cache_seq_stride < head_dim)
-        return NK_ERR_SHAPE;
+    if (!q || !c || !c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale || !position || !out)
+        return NK_ERR_ARG;
+    if (!q8_cache_ok(c, tokens, q_heads)) return NK_ERR_SHAPE;
     Q8AttnArgs a{};
-    a.G = q_heads / kv_heads;
+    a.G = q_heads / c->kv_heads;
     a.rows = q8_rows(tokens * a.G);
     a.row_blocks = (tokens * a.G + a.rows - 1) / a.rows;
     // units of the whole launch are counted in 32 bits
-    if ((int64_t)((capacity + kQ8Unit - 1) / kQ8Unit) * batch * kv_heads * a.row_blocks > (1 << 30))
+    if ((int64_t)((c->capacity + kQ8Unit - 1) / kQ8Unit) * c->batch * c->kv_heads * a.row_blocks >
+        (1 << 30))
         return NK_ERR_SHAPE;
-    if (!ws || ws_bytes < nk_attention_q8_ws_bytes(tokens, q_heads, kv_heads))
+    if (!ws || ws_bytes < nk_attention_q8_ws_bytes(tokens, q_heads, c->kv_heads))
         return NK_ERR_WORKSPACE;
-    if ((((uintptr_t)q | (uintptr_t)position | (uintptr_t)out) & 7u) ||
-        (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)ws) & 15u) ||
-        (((uintptr_t)k_scale | (uintptr_t)v_scale) & 3u) || cache_batch_stride % 16 ||
-        cache_head_stride % 16 || cache_seq_stride % 16)
+    if ((((uintptr_t)q | (uintptr_t)position | (uintptr_t)out) & 7u) || ((uintptr_t)ws & 15u) ||
+        !q8_cache_aligned(c))
         return NK_ERR_ALIGN;
     a.q = static_cast<const __nv_bfloat16*>(q);
-    a.k = static_cast<const uint8_t*>(k_codes);
-    a.v = static_cast<const uint8_t*>(v_codes);
-    a.ks = k_scale;
-    a.vs = v_scale;
+    a.k = static_cast<const uint8_t*>(c->k_codes);
+    a.v = static_cast<const uint8_t*>(c->v_codes);
+    a.ks = c->k_scale;
+    a.vs = c->v_scale;
     a.position = position;
     a.per_sequence = per_sequence != 0;
     a.out = static_cast<__nv_bfloat16*>(out);
     a.part = static_cast<float*>(ws);
-    a.batch = batch;
+    a.batch = c->batch;
     a.tokens = tokens;
     a.hq = q_heads;
-    a.hkv = kv_heads;
-    a.capacity = capacity;
-    a.lg_block = __builtin_ctz(block);
-    a.blocks = (capacity + block - 1) / block;
-    a.cb = cache_batch_stride;
-    a.ch = cache_head_stride;
-    a.cs = cache_seq_stride;
+    a.hkv = c->kv_heads;
+    a.capacity = c->capacity;
+    a.lg_block = __builtin_ctz(c->block);
+    a.g_mul = (65536 + a.G - 1) / a.G;  // r / G for the at most 256 rows of a pair
+    a.blocks = (c->capacity + c->block - 1) / c->block;
+    a.cb = c->batch_stride;
+    a.ch = c->head_stride;
+    a.cs = c->seq_stride;
     a.scale_log2 = scale * 1.4426950408889634f;
     cudaStream_t s = (cudaStream_t)stream;
     switch (a.rows) {
         case 8: return q8_launch_attn<1>(a, s);
-        case 16: return q8_launch_attn<2>(a, s);
-        default: return q8_launch_attn<4>(a, s);
+        default: return q8_launch_attn<2>(a, s);
     }
 }

@@ -655,23 +655,23 @@ extern "C" size_t nk_w4_zero_bytes(int N, int K, int group) {
     return nk_w4_scale_bytes(N, K, group) / 2;
 }
 
-extern "C" int nk_gemm_w4(const void* x, int64_t ldx, const void* codes, const void* scales,
-                          const void* zeros, void* y, int64_t ldy, int M, int N, int K, int group,
-                          int scale_type, nk_stream_t stream) {
+extern "C" int nk_gemm_w4(const void* x, int64_t ldx, const nk_w4_weight* w, void* y, int64_t ldy,
+                          int M, nk_stream_t stream) {
     using namespace nk;
-    if (!x || !codes || !scales || !y) return NK_ERR_ARG;
-    if (scale_type != NK_W4_SCALE_BF16 && scale_type != NK_W4_SCALE_FP16) return NK_ERR_ARG;
+    if (!x || !w || !w->codes || !w->scales || !y) return NK_ERR_ARG;
+    const int N = w->N, K = w->K, group = w->group;
+    if (w->scale_type != NK_W4_SCALE_BF16 && w->scale_type != NK_W4_SCALE_FP16) return NK_ERR_ARG;
     if (!w4_shape_ok(N, K) || !w4_group_ok(group) || M < 1 || M > (1 << 20) || ldx < K || ldy < N)
         return NK_ERR_SHAPE;
-    if ((((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)zeros) & 15u) ||
+    if ((((uintptr_t)w->codes | (uintptr_t)w->scales | (uintptr_t)w->zeros) & 15u) ||
         (((uintptr_t)x | (uintptr_t)y) & 1u))
         return NK_ERR_ALIGN;
     W4Args a{};
     a.x = static_cast<const __nv_bfloat16*>(x);
     a.ldx = M == 1 ? (K + 7) / 8 * 8 : ldx;  // (one row: any stride)
-    a.codes = static_cast<const uint8_t*>(codes);
-    a.scales = static_cast<const uint8_t*>(scales);
-    a.zeros = static_cast<const uint8_t*>(zeros);
+    a.codes = static_cast<const uint8_t*>(w->codes);
+    a.scales = static_cast<const uint8_t*>(w->scales);
+    a.zeros = static_cast<const uint8_t*>(w->zeros);
     a.y = static_cast<__nv_bfloat16*>(y);
     a.ldy = ldy;
     a.M = M;
@@ -679,7 +679,7 @@ extern "C" int nk_gemm_w4(const void* x, int64_t ldx, const void* codes, const v
     a.K = K;
     a.KB = (K + 127) / 128;
     a.wide_x = ((uintptr_t)x & 15u) == 0 && a.ldx % 8 == 0;
-    const bool fp16 = scale_type == NK_W4_SCALE_FP16;
+    const bool fp16 = w->scale_type == NK_W4_SCALE_FP16;
     cudaStream_t s = (cudaStream_t)stream;
     if (M <= 16) return w4_dispatch<16>(a, group, fp16, s);
     if (M <= 32) return w4_dispatch<32>(a, group, fp16, s);

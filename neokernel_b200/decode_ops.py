@@ -24,6 +24,7 @@ Both take per-sequence positions, idle sequences and up to 16 new tokens a seque
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -168,7 +169,7 @@ class Q8Cache:
     contiguous. The tensors are the caller's and are read and written in place."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "block", "batch", "kv_heads", "capacity",
-                 "device", "_ptrs", "_dims")
+                 "device", "_c", "_addr")
 
     def __init__(self, k, v, k_scale, v_scale, block: int):
         for t in (k, v):
@@ -198,9 +199,10 @@ class Q8Cache:
                   f"Q8Cache: scales must be contiguous fp32 {list(shape)} on the codes' device")
         self.k, self.v, self.k_scale, self.v_scale, self.block = k, v, k_scale, v_scale, block
         self.batch, self.kv_heads, self.capacity, self.device = B, H, S, k.device
-        self._ptrs = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
-        strides = (sb if B > 1 else 0, sh if H > 1 else 0, ss if S > 1 else HEAD_DIM)
-        self._dims = (HEAD_DIM, S, block, *strides)
+        self._c = _lib.NkQ8Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                 B, H, HEAD_DIM, S, block, 0, sb if B > 1 else 0,
+                                 sh if H > 1 else 0, ss if S > 1 else HEAD_DIM)
+        self._addr = ctypes.addressof(self._c)
 
     @classmethod
     def empty(cls, batch: int, kv_heads: int, capacity: int, device, block: int = 64,
@@ -237,31 +239,39 @@ class Q8Cache:
         return full(self.k, self.k_scale), full(self.v, self.v_scale)
 
 
-def _q8_rows(x, cache, width, name):
-    """(tokens per sequence, row stride) of a [batch * tokens, width] bf16 operand."""
-    _need(isinstance(x, torch.Tensor) and x.dtype is torch.bfloat16 and x.device == cache.device
-          and x.dim() == 2, f"{name} must be a 2-D bf16 tensor on the cache's device")
-    rows = x.shape[0]
-    T = rows // cache.batch
-    _need(x.shape[1] == width and T * cache.batch == rows and 1 <= T <= Q8_MAX_TOKENS
-          and T <= cache.capacity,
-          f"{name} must be [batch * tokens, {width}] for batch {cache.batch}, tokens 1.."
-          f"{Q8_MAX_TOKENS} within the capacity {cache.capacity}, got {list(x.shape)}")
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(dev).cuda_stream, without the object
+_BF16, _INT64 = torch.bfloat16, torch.int64
+
+
+def _q8_tokens(x, cache, width, name):
+    """New tokens per sequence of a [batch * tokens, width] bf16 operand."""
+    if not (isinstance(x, torch.Tensor) and x.dtype is _BF16 and x.dim() == 2
+            and x.device == cache.device):
+        raise ValueError(f"{name} must be a 2-D bf16 tensor on the cache's device")
+    rows, cols = x.shape
+    T, rest = divmod(rows, cache.batch)
+    if rest or cols != width or not 1 <= T <= Q8_MAX_TOKENS or T > cache.capacity:
+        raise ValueError(f"{name} must be [batch * tokens, {width}] for batch {cache.batch}, tokens "
+                         f"1..{Q8_MAX_TOKENS} within the capacity {cache.capacity}, got "
+                         f"[{rows}, {cols}]")
     return T
 
 
 def _q8_position(position, cache, name):
     """1 if the int64 ``position`` has an entry per sequence, 0 if one for all."""
-    _need(isinstance(position, torch.Tensor) and position.dtype is torch.int64
-          and position.device == cache.device and position.is_contiguous()
-          and position.numel() in (1, cache.batch) and position.dim() == 1,
-          f"{name}: position must be a contiguous int64 tensor [1] or [{cache.batch}] on the "
-          "cache's device")
-    return 1 if position.numel() == cache.batch else 0
+    if (isinstance(position, torch.Tensor) and position.dtype is _INT64 and position.dim() == 1
+            and position.device == cache.device and position.is_contiguous()):
+        n = position.numel()
+        if n == cache.batch:
+            return 1
+        if n == 1:
+            return 0
+    raise ValueError(f"{name}: position must be a contiguous int64 tensor [1] or [{cache.batch}] on "
+                     "the cache's device")
 
 
 def _on(device, fn, args):
-    if device.index != torch.cuda.current_device():
+    if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return fn(*args)
     return fn(*args)
@@ -276,33 +286,36 @@ def qk_norm_rope_cache_q8(qkv, q_norm, k_norm, cos, sin, position, q_out, cache:
     sequence, of which nothing is read or written. q_out [batch * T, heads * 128] contiguous. A
     block's scale is the smallest power of two that keeps its new tokens within e4m3's range,
     and at least its former one where it holds earlier tokens; these are rounded anew when it
-    rises. A position past capacity - T is an idle sequence too and is reported by ``device_error()``."""
+    rises. A position past capacity - T is an idle sequence too and is reported by
+    ``device_error()``. ``heads`` is 1 to 16 times the cache's kv_heads."""
     name = "qk_norm_rope_cache_q8"
-    H, Hkv = int(heads), cache.kv_heads
-    _need(H >= 1 and H % Hkv == 0, f"{name}: heads must be a multiple of the cache's {Hkv}")
-    T = _q8_rows(qkv, cache, (H + 2 * Hkv) * HEAD_DIM, f"{name}: qkv")
-    _need(_q8_rows(q_out, cache, H * HEAD_DIM, f"{name}: q_out") == T and q_out.is_contiguous(),
-          f"{name}: q_out must be contiguous, with as many rows as qkv")
+    Hkv, dev = cache.kv_heads, cache.device
+    T = _q8_tokens(qkv, cache, (heads + 2 * Hkv) * HEAD_DIM, "qk_norm_rope_cache_q8: qkv")
+    if _q8_tokens(q_out, cache, heads * HEAD_DIM, "qk_norm_rope_cache_q8: q_out") != T \
+            or not q_out.is_contiguous():
+        raise ValueError(f"{name}: q_out must be contiguous, with as many rows as qkv")
     per = _q8_position(position, cache, name)
-    st = qkv.stride()
-    ld = st[0] if qkv.shape[0] > 1 else qkv.shape[1]
-    _need(st[1] == 1 and ld >= qkv.shape[1] and ld % 4 == 0 and qkv.data_ptr() % 8 == 0
-          and q_out.data_ptr() % 8 == 0,
-          f"{name}: qkv rows must have unit column stride, 8-byte aligned")
-    for t, shape in ((q_norm, (HEAD_DIM,)), (k_norm, (HEAD_DIM,))):
-        _need(isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.shape == shape
-              and t.device == cache.device and t.stride(0) == 1 and t.data_ptr() % 8 == 0,
-              f"{name}: q_norm and k_norm must be bf16 [128] on the cache's device")
+    ld, unit = qkv.stride()
+    if T * cache.batch == 1:
+        ld = qkv.shape[1]
+    if unit != 1 or ld < qkv.shape[1]:
+        raise ValueError(f"{name}: qkv rows must have unit column stride and not overlap")
+    for t in (q_norm, k_norm):
+        if not (isinstance(t, torch.Tensor) and t.dtype is _BF16 and t.device == dev
+                and t.shape == (HEAD_DIM,) and t.is_contiguous()):
+            raise ValueError(f"{name}: q_norm and k_norm must be contiguous bf16 [128] on the "
+                             "cache's device")
     for t in (cos, sin):
-        _need(isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.dim() == 2
-              and t.shape[0] >= cache.capacity and t.shape[1] == HEAD_DIM and t.is_contiguous()
-              and t.device == cache.device and t.data_ptr() % 8 == 0,
-              f"{name}: cos and sin must be contiguous bf16 [capacity, 128] on the cache's device")
-    status = _on(cache.device, _lib.load().nk_qk_norm_rope_cache_q8, (
+        if not (isinstance(t, torch.Tensor) and t.dtype is _BF16 and t.device == dev
+                and t.dim() == 2 and t.shape[1] == HEAD_DIM and t.shape[0] >= cache.capacity
+                and t.is_contiguous()):
+            raise ValueError(f"{name}: cos and sin must be contiguous bf16 [capacity, 128] on the "
+                             "cache's device")
+    status = _on(dev, _lib.load().nk_qk_norm_rope_cache_q8, (
         qkv.data_ptr(), ld, q_norm.data_ptr(), k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-        position.data_ptr(), per, q_out.data_ptr(), *cache._ptrs, cache.batch, T, H, Hkv,
-        *cache._dims, float(eps), _stream(qkv)))
-    if status != _lib.NK_OK:
+        position.data_ptr(), per, q_out.data_ptr(), cache._addr, T, heads, eps,
+        _raw_stream(dev.index)))
+    if status:
         _raise(status, "nk_qk_norm_rope_cache_q8")
     return q_out
 
@@ -318,6 +331,9 @@ def attention_q8_workspace(cache: Q8Cache, heads: int, tokens: int = 1) -> torch
     return torch.empty(n, dtype=torch.uint8, device=cache.device)
 
 
+_ATTN_SCALE = 1.0 / math.sqrt(HEAD_DIM)
+
+
 def attention_decode_q8(q, cache: Q8Cache, position, out, ws, heads: int,
                         scale: float | None = None):
     """``attention_decode`` of T = 1..16 new tokens per sequence over a ``Q8Cache`` that already
@@ -325,21 +341,17 @@ def attention_decode_q8(q, cache: Q8Cache, position, out, ws, heads: int,
     [0, position[b] + t]. ``position`` as in ``qk_norm_rope_cache_q8``; rows of idle sequences
     come out zero. ``heads`` is 1 to 16 times the cache's kv_heads."""
     name = "attention_decode_q8"
-    H = int(heads)
-    _need(H >= 1 and H % cache.kv_heads == 0 and H // cache.kv_heads <= 16,
-          f"{name}: heads must be 1 to 16 times the cache's {cache.kv_heads}")
-    T = _q8_rows(q, cache, H * HEAD_DIM, f"{name}: q")
-    _need(_q8_rows(out, cache, H * HEAD_DIM, f"{name}: out") == T and q.is_contiguous()
-          and out.is_contiguous() and q.data_ptr() % 8 == 0 and out.data_ptr() % 8 == 0,
-          f"{name}: q and out must be contiguous, 8-byte aligned and of the same shape")
+    T = _q8_tokens(q, cache, heads * HEAD_DIM, "attention_decode_q8: q")
+    if _q8_tokens(out, cache, heads * HEAD_DIM, "attention_decode_q8: out") != T \
+            or not (q.is_contiguous() and out.is_contiguous()):
+        raise ValueError(f"{name}: q and out must be contiguous and of the same shape")
     per = _q8_position(position, cache, name)
-    _need(isinstance(ws, torch.Tensor) and ws.device == cache.device and ws.is_contiguous(),
-          f"{name}: ws must be a workspace on the cache's device")
-    scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
+    if not (isinstance(ws, torch.Tensor) and ws.device == cache.device and ws.is_contiguous()):
+        raise ValueError(f"{name}: ws must be a workspace on the cache's device")
     status = _on(cache.device, _lib.load().nk_attention_decode_q8, (
-        q.data_ptr(), *cache._ptrs, position.data_ptr(), per, out.data_ptr(), cache.batch, T, H,
-        cache.kv_heads, *cache._dims, scale, ws.data_ptr(), ws.numel() * ws.element_size(),
-        _stream(q)))
-    if status != _lib.NK_OK:
+        q.data_ptr(), cache._addr, position.data_ptr(), per, out.data_ptr(), T, heads,
+        _ATTN_SCALE if scale is None else scale, ws.data_ptr(), ws.nbytes,
+        _raw_stream(cache.device.index)))
+    if status:
         _raise(status, "nk_attention_decode_q8")
     return out

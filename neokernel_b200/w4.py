@@ -12,6 +12,8 @@ workspace.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -33,14 +35,17 @@ class W4Weight:
     reads them ahead of the work queued before it on its stream.
     """
 
-    __slots__ = ("N", "K", "group", "codes", "scales", "zeros", "scale_type", "device", "_args")
+    __slots__ = ("N", "K", "group", "codes", "scales", "zeros", "scale_type", "device", "_c",
+                 "_addr")
 
     def __init__(self, N, K, group, codes, scales, zeros, scale_type):
         self.N, self.K, self.group = N, K, group
         self.codes, self.scales, self.zeros, self.scale_type = codes, scales, zeros, scale_type
         self.device = codes.device
-        self._args = (codes.data_ptr(), scales.data_ptr(),
-                      zeros.data_ptr() if zeros is not None else None)
+        self._c = _lib.NkW4Weight(codes.data_ptr(), scales.data_ptr(),
+                                  zeros.data_ptr() if zeros is not None else None, N, K, group,
+                                  scale_type)
+        self._addr = ctypes.addressof(self._c)
 
     @property
     def shape(self):
@@ -142,6 +147,7 @@ class W4Weight:
 
 
 _BF16 = torch.bfloat16
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(dev).cuda_stream, without the object
 
 
 def mm_w4(a: torch.Tensor, w: W4Weight, *, out: torch.Tensor,
@@ -154,9 +160,9 @@ def mm_w4(a: torch.Tensor, w: W4Weight, *, out: torch.Tensor,
     """
     if not isinstance(w, W4Weight):
         raise ValueError(f"mm_w4: w must be a W4Weight, got {type(w).__name__}")
-    for t, name in ((a, "a"), (out, "out")):
-        if not isinstance(t, torch.Tensor) or t.dtype is not _BF16 or t.dim() != 2:
-            raise ValueError(f"mm_w4: {name} must be a 2-D bfloat16 tensor")
+    if not (isinstance(a, torch.Tensor) and isinstance(out, torch.Tensor) and a.dtype is _BF16
+            and out.dtype is _BF16 and a.dim() == 2 and out.dim() == 2):
+        raise ValueError("mm_w4: a and out must be 2-D bfloat16 tensors")
     dev = w.device
     if not a.is_cuda or a.device != dev or out.device != dev:
         raise ValueError(f"mm_w4: a, w and out must be on the same CUDA device (a on {a.device}, "
@@ -165,29 +171,26 @@ def mm_w4(a: torch.Tensor, w: W4Weight, *, out: torch.Tensor,
     N = w.N
     if K != w.K:
         raise ValueError(f"mm_w4: a is [{M}, {K}] but w is [{w.K}, {N}]")
-    if tuple(out.shape) != (M, N):
+    if out.shape != (M, N):
         raise ValueError(f"mm_w4: out must be [{M}, {N}], got {tuple(out.shape)}")
     if M == 0:
         return out
-    ldx, ldy = K, N
-    sa, so = a.stride(), out.stride()
-    if (sa[1] != 1 and K > 1) or (so[1] != 1 and N > 1):
+    ldx, ca = a.stride()
+    ldy, co = out.stride()
+    if (ca != 1 and K > 1) or (co != 1 and N > 1):
         raise ValueError("mm_w4: a and out must have unit stride along their last dimension")
-    if M > 1:
-        ldx, ldy = sa[0], so[0]
-        if ldx < K or ldy < N:
-            raise ValueError("mm_w4: rows of a and of out must not overlap")
-    cs, ss, zs = w._args
-    if stream is None:
-        stream = torch.cuda.current_stream(dev)
-    L = _lib.load()
-    args = (a.data_ptr(), ldx, cs, ss, zs, out.data_ptr(), ldy, M, N, K, w.group, w.scale_type,
-            stream.cuda_stream)
-    if dev.index != torch.cuda.current_device():
+    if M == 1:
+        ldx, ldy = K, N
+    elif ldx < K or ldy < N:
+        raise ValueError("mm_w4: rows of a and of out must not overlap")
+    index = dev.index
+    handle = _raw_stream(index) if stream is None else stream.cuda_stream
+    fn = _lib.load().nk_gemm_w4
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
-            status = L.nk_gemm_w4(*args)
+            status = fn(a.data_ptr(), ldx, w._addr, out.data_ptr(), ldy, M, handle)
     else:
-        status = L.nk_gemm_w4(*args)
-    if status != _lib.NK_OK:
+        status = fn(a.data_ptr(), ldx, w._addr, out.data_ptr(), ldy, M, handle)
+    if status:
         _raise(status, f"nk_gemm_w4(M={M}, N={N}, K={K})")
     return out

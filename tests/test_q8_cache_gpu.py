@@ -82,6 +82,9 @@ def run_attention(q, cache, pos, heads, scale=None, out=None):
     out = torch.full_like(q, float("nan")) if out is None else out
     position = torch.tensor(pos, device=DEV)
     assert ops.attention_decode_q8(q, cache, position, out, ws, heads, scale) is out
+    again = torch.full_like(q, float("nan"))  # with the workspace as the first call left it
+    ops.attention_decode_q8(q, cache, position, again, ws, heads, scale)
+    assert torch.equal(out.view(torch.int16), again.view(torch.int16))
     return out
 
 

@@ -97,43 +97,56 @@ def test_w4_sizes_out_of_range():
 
 def test_gemm_w4_abi_refusals():
     L = _lib.load()
-    p = ctypes.c_void_p(1 << 20)  # aligned and never read: every call is refused
+    p = 1 << 20  # aligned and never read: every call is refused
+    ok = dict(x=p, ldx=256, codes=p, scales=p, zeros=None, y=p, ldy=64, M=1, N=64, K=256, group=128,
+              st=0)
 
-    def call(x=p, ldx=256, codes=p, scales=p, zeros=None, y=p, ldy=64, M=1, N=64, K=256, group=128,
-             st=0):
-        return L.nk_gemm_w4(x, ldx, codes, scales, zeros, y, ldy, M, N, K, group, st, None)
+    def call(**kw):
+        v = ok | kw
+        w = _lib.NkW4Weight(v["codes"], v["scales"], v["zeros"], v["N"], v["K"], v["group"], v["st"])
+        return L.nk_gemm_w4(v["x"], v["ldx"], ctypes.addressof(w), v["y"], v["ldy"], v["M"], None)
 
-    at = lambda n: ctypes.c_void_p((1 << 20) + n)  # noqa: E731
+    assert L.nk_gemm_w4(p, 256, None, p, 64, 1, None) == _lib.NK_ERR_ARG
     for kw in (dict(x=None), dict(codes=None), dict(scales=None), dict(y=None), dict(st=2),
                dict(st=-1)):
         assert call(**kw) == _lib.NK_ERR_ARG, kw
     for kw in (dict(M=0), dict(M=-1), dict(M=(1 << 20) + 1), dict(N=0), dict(K=0), dict(group=16),
                dict(group=0), dict(ldx=255), dict(ldy=63), dict(N=(1 << 24) + 1)):
         assert call(**kw) == _lib.NK_ERR_SHAPE, kw
-    for kw in (dict(codes=at(8)), dict(scales=at(2)), dict(zeros=at(4)), dict(x=at(1)),
-               dict(y=at(1))):
+    for kw in (dict(codes=p + 8), dict(scales=p + 2), dict(zeros=p + 4), dict(x=p + 1),
+               dict(y=p + 1)):
         assert call(**kw) == _lib.NK_ERR_ALIGN, kw
+
+
+CACHE = dict(k=1 << 20, v=1 << 20, ks=1 << 20, vs=1 << 20, batch=2, hkv=8, d=128, cap=64, block=16,
+             reserved=0, cb=8 * 64 * 128, ch=64 * 128, cs=128)
+BAD_SHAPES = (dict(batch=0), dict(batch=1025), dict(tokens=0), dict(tokens=17), dict(hq=0),
+              dict(hkv=0), dict(hq=33), dict(hq=136), dict(d=64), dict(cap=0),
+              dict(cap=(1 << 30) + 1), dict(tokens=16, cap=15), dict(block=8), dict(block=48),
+              dict(block=256), dict(cs=112))
+BAD_ALIGNMENT = (dict(k=(1 << 20) + 8), dict(v=(1 << 20) + 4), dict(ks=(1 << 20) + 2),
+                 dict(vs=(1 << 20) + 1), dict(pos=(1 << 20) + 4), dict(cs=136),
+                 dict(ch=64 * 128 + 8), dict(cb=8 * 64 * 128 + 4))
 
 
 def test_append_q8_abi_refusals():
     L = _lib.load()
     p = 1 << 20
-    ok = dict(qkv=p, ld=48 * 128, qn=p, kn=p, cos=p, sin=p, pos=p, per=1, q=p, k=p, v=p, ks=p, vs=p,
-              batch=2, tokens=1, hq=32, hkv=8, d=128, cap=64, block=16, cb=8 * 64 * 128,
-              ch=64 * 128, cs=128, eps=1e-6, stream=None)
+    ok = dict(qkv=p, ld=48 * 128, qn=p, kn=p, cos=p, sin=p, pos=p, per=1, q=p, tokens=1, hq=32)
 
     def call(**kw):
-        return L.nk_qk_norm_rope_cache_q8(*(ok | kw).values())
+        v = ok | kw
+        c = _lib.NkQ8Cache(*(kw.get(n, x) for n, x in CACHE.items()))
+        return L.nk_qk_norm_rope_cache_q8(
+            v["qkv"], v["ld"], v["qn"], v["kn"], v["cos"], v["sin"], v["pos"], v["per"], v["q"],
+            kw.get("cache", ctypes.addressof(c)), v["tokens"], v["hq"], 1e-6, None)
 
-    for n in ("qkv", "qn", "kn", "cos", "sin", "pos", "q", "k", "v", "ks", "vs"):
+    for n in ("qkv", "qn", "kn", "cos", "sin", "pos", "q", "k", "v", "ks", "vs", "cache"):
         assert call(**{n: None}) == _lib.NK_ERR_ARG, n
-    for kw in (dict(batch=0), dict(batch=1025), dict(tokens=0), dict(tokens=17), dict(hq=0),
-               dict(hkv=0), dict(hq=33), dict(d=64), dict(cap=0), dict(tokens=16, cap=15),
-               dict(block=8), dict(block=48), dict(block=256), dict(ld=48 * 128 - 4), dict(cs=64)):
+    for kw in BAD_SHAPES + (dict(ld=48 * 128 - 4),):
         assert call(**kw) == _lib.NK_ERR_SHAPE, kw
-    for kw in (dict(qkv=p + 4), dict(q=p + 2), dict(k=p + 8), dict(v=p + 4), dict(ks=p + 2),
-               dict(pos=p + 4), dict(ld=48 * 128 + 2), dict(cs=136), dict(ch=64 * 128 + 8),
-               dict(cb=8 * 64 * 128 + 4), dict(cos=p + 2)):
+    for kw in BAD_ALIGNMENT + (dict(qkv=p + 4), dict(q=p + 2), dict(ld=48 * 128 + 2),
+                               dict(cos=p + 2)):
         assert call(**kw) == _lib.NK_ERR_ALIGN, kw
 
 
@@ -142,23 +155,22 @@ def test_attention_q8_abi_refusals():
     p = 1 << 20
     need = L.nk_attention_q8_ws_bytes(1, 32, 8)
     assert need > 0
-    ok = dict(q=p, k=p, v=p, ks=p, vs=p, pos=p, per=0, out=p, batch=2, tokens=1, hq=32, hkv=8,
-              d=128, cap=64, block=64, cb=8 * 64 * 128, ch=64 * 128, cs=128, scale=0.1, ws=p,
-              n=need, stream=None)
+    ok = dict(q=p, pos=p, per=0, out=p, tokens=1, hq=32, ws=p, n=need)
 
     def call(**kw):
-        return L.nk_attention_decode_q8(*(ok | kw).values())
+        v = ok | kw
+        c = _lib.NkQ8Cache(*(kw.get(n, x) for n, x in CACHE.items()))
+        return L.nk_attention_decode_q8(v["q"], kw.get("cache", ctypes.addressof(c)), v["pos"],
+                                        v["per"], v["out"], v["tokens"], v["hq"], 0.1, v["ws"],
+                                        v["n"], None)
 
-    for n in ("q", "k", "v", "ks", "vs", "pos", "out"):
+    for n in ("q", "k", "v", "ks", "vs", "pos", "out", "cache"):
         assert call(**{n: None}) == _lib.NK_ERR_ARG, n
-    for kw in (dict(batch=0), dict(batch=1025), dict(tokens=0), dict(tokens=17), dict(hkv=0),
-               dict(hq=33), dict(hq=136), dict(d=64), dict(cap=0), dict(tokens=2, cap=1),
-               dict(block=1), dict(cs=112), dict(cap=2 ** 31 - 1, batch=1024)):
+    for kw in BAD_SHAPES + (dict(cap=1 << 30, batch=1024),):
         assert call(**kw) == _lib.NK_ERR_SHAPE, kw
     for kw in (dict(ws=None), dict(n=need - 1), dict(tokens=16)):
         assert call(**kw) == _lib.NK_ERR_WORKSPACE, kw
-    for kw in (dict(q=p + 4), dict(out=p + 2), dict(k=p + 8), dict(v=p + 1), dict(ws=p + 8),
-               dict(ks=p + 1), dict(cs=130), dict(ch=4), dict(cb=12), dict(pos=p + 4)):
+    for kw in BAD_ALIGNMENT + (dict(q=p + 4), dict(out=p + 2), dict(ws=p + 8)):
         assert call(**kw) == _lib.NK_ERR_ALIGN, kw
 
 
