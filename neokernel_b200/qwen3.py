@@ -36,6 +36,10 @@ Weights are random and seeded; no checkpoint is used. Two initialisations (``ini
   154-156): ``normal_(0, 0.02)`` for every matrix and ones for the norm gains. Its logits are
   nearly flat (top-2 gaps of a few hundredths), so greedy tokens flip on genuine near-ties
   between any two valid fp32-accumulating GEMMs.
+
+The fused step also runs with its two byte streams quantised, either or both: the four layer
+linears in 4 bits (``quantize_linears``, with ``linear=w4.linear``; lm_head stays bf16) and the
+KV cache in 8 bits (``cache="e4m3"``, decode_ops.Q8Cache).
 """
 
 from __future__ import annotations
@@ -79,6 +83,7 @@ QWEN3_32B = Qwen3Dims(5120, 25600, 64, 8, 128, 64, 151936)
 
 
 INITS = ("decisive", "reference")
+CACHES = ("bf16", "e4m3")
 
 # True: the fused decode step runs the QKV linear and its q/k-norm + RoPE + cache consumer as
 # one launch (nk_gemm_bf16_qkv_rope_cache) when the linear is neokernel_b200.mm. Off by
@@ -162,6 +167,33 @@ class Qwen3Weights:
         self.lm_head = self.lm_head_weight.t()  # engine/engine.py:70
 
 
+class W4LayerWeights:
+    """A layer with its four linears as ``w4.W4Weight``; norm gains shared with ``lw``."""
+
+    def __init__(self, lw: LayerWeights, group: int, zeros: bool):
+        from .w4 import W4Weight
+        for name in ("qkv", "o", "gate_up", "down"):
+            setattr(self, name, W4Weight.quantize(getattr(lw, name + "_weight"), group, zeros=zeros))
+        self.input_norm, self.post_norm = lw.input_norm, lw.post_norm
+        self.q_norm, self.k_norm = lw.q_norm, lw.k_norm
+
+
+class Qwen3W4Weights:
+    """``w`` with every layer's linears in 4 bits; embedding, norms and lm_head are ``w``'s own."""
+
+    def __init__(self, w: Qwen3Weights, group: int, zeros: bool):
+        self.dims, self.init = w.dims, w.init
+        self.embed, self.final_norm = w.embed, w.final_norm
+        self.lm_head_weight, self.lm_head = w.lm_head_weight, w.lm_head
+        self.layers = [W4LayerWeights(lw, group, zeros) for lw in w.layers]
+
+
+def quantize_linears(w: Qwen3Weights, group: int = 128, zeros: bool = False) -> Qwen3W4Weights:
+    """The model with its layer linears rounded to 4 bits (scales in bf16 per ``group`` of K, and
+    with ``zeros`` a zero point each). Decode it with ``linear=w4.linear, fused=True``."""
+    return Qwen3W4Weights(w, group, zeros)
+
+
 def rope_tables(d: Qwen3Dims, capacity: int, device):
     """Rotary cos/sin [capacity, head_dim] in bf16 (Qwen3 rotary embedding: inverse
     frequencies theta^(-2i/D) in fp32, angles duplicated across the two halves)."""
@@ -189,9 +221,14 @@ def rotate_half(x):
 
 class DecodeState:
     """Fixed buffers for batch ``B`` and cache ``capacity`` (reference: DecodeBuffers,
-    engine/kernels/decode.py:10-39, and Engine.prepare, engine/engine.py:76-98)."""
+    engine/kernels/decode.py:10-39, and Engine.prepare, engine/engine.py:76-98). ``cache``:
+    "bf16", or "e4m3" for 8-bit caches (``q8``, one decode_ops.Q8Cache per layer; the fused
+    step)."""
 
-    def __init__(self, w: Qwen3Weights, batch: int, capacity: int, device="cuda"):
+    def __init__(self, w: Qwen3Weights, batch: int, capacity: int, device="cuda",
+                 cache: str = "bf16"):
+        if cache not in CACHES:
+            raise ValueError(f"cache must be one of {CACHES}, not {cache!r}")
         d = w.dims
         bf = dict(device=device, dtype=torch.bfloat16)
         self.batch, self.capacity = batch, capacity
@@ -207,6 +244,11 @@ class DecodeState:
         self.logits = torch.empty(batch, d.vocab, **bf)
         self.next_tokens = torch.zeros(batch, device=device, dtype=torch.int64)
         n = len(w.layers)
+        self.q8 = None
+        if cache == "e4m3":
+            from .decode_ops import Q8Cache
+            self.q8 = [Q8Cache.empty(batch, d.kv_heads, capacity, device) for _ in range(n)]
+        n = 0 if self.q8 else n
         self.k_cache = [torch.zeros(batch, d.kv_heads, capacity, d.head_dim, **bf) for _ in range(n)]
         self.v_cache = [torch.zeros(batch, d.kv_heads, capacity, d.head_dim, **bf) for _ in range(n)]
         self.cos, self.sin = rope_tables(d, capacity, device)
@@ -260,15 +302,20 @@ def layer_step(st: DecodeState, w: LayerWeights, k_cache, v_cache, d: Qwen3Dims,
 
 
 def layer_step_fused(st: DecodeState, w: LayerWeights, k_cache, v_cache, d: Qwen3Dims, linear,
-                     row_linear=None, carry=False):
+                     row_linear=None, carry=False, q8=None):
     """The same layer on the fused kernels (neokernel_b200.decode_ops), with the reference's
     fuse_norm_residual scheme (engine/kernels/decode.py:42-68): the down projection's output
-    stays in ``branch`` and the next RMSNorm adds it into ``x`` (``carry``)."""
+    stays in ``branch`` and the next RMSNorm adds it into ``x`` (``carry``). ``q8``: the layer's
+    8-bit cache, in place of ``k_cache`` and ``v_cache``."""
     from . import decode_ops as ops
     from . import gemm
     row_linear = row_linear or linear
     ops.rmsnorm(st.x, w.input_norm, st.norm, d.eps, branch=st.branch if carry else None)
-    if FUSE_QKV and linear is gemm.mm and st.batch <= 16:
+    if q8 is not None:
+        linear(st.norm, w.qkv, out=st.qkv)
+        ops.qk_norm_rope_cache_q8(st.qkv, w.q_norm, w.k_norm, st.cos, st.sin, st.position, st.q, q8,
+                                  d.heads, d.eps)
+    elif FUSE_QKV and linear is gemm.mm and st.batch <= 16:
         # decode.py:54-55 in one launch: the QKV linear finishes each head with its norm, RoPE
         # and cache write (qkv is not stored)
         ops.qkv_rope_cache(st.norm, w.qkv, w.q_norm, w.k_norm, st.cos, st.sin, st.position,
@@ -277,8 +324,11 @@ def layer_step_fused(st: DecodeState, w: LayerWeights, k_cache, v_cache, d: Qwen
         linear(st.norm, w.qkv, out=st.qkv)                               # decode.py:54
         ops.qk_norm_rope_cache(st.qkv, w.q_norm, w.k_norm, st.cos, st.sin, st.position, st.q,
                                k_cache, v_cache, d.heads, d.kv_heads, d.eps)
-    ops.attention_decode(st.q, k_cache, v_cache, st.position, st.attn, st.attn_ws,
-                         d.heads, d.kv_heads)
+    if q8 is not None:
+        ops.attention_decode_q8(st.q, q8, st.position, st.attn, st.attn_ws, d.heads)
+    else:
+        ops.attention_decode(st.q, k_cache, v_cache, st.position, st.attn, st.attn_ws,
+                             d.heads, d.kv_heads)
     row_linear(st.attn, w.o, out=st.branch)                              # decode.py:58
     ops.rmsnorm(st.x, w.post_norm, st.norm, d.eps, branch=st.branch)
     linear(st.norm, w.gate_up, out=st.gate_up)                           # decode.py:64
@@ -307,14 +357,20 @@ def decode_step(st: DecodeState, w: Qwen3Weights, linear, row_linear=None, head=
     tensor-parallel mode replaces (neokernel_b200.tp); by default the step is single-GPU.
     ``fused`` runs the non-linear ops on the fused CUDA kernels instead of PyTorch ops."""
     d = w.dims
+    if st.q8 is not None and not fused:
+        raise ValueError("an 8-bit cache needs the fused step")
     torch.index_select(w.embed, 0, st.tokens, out=st.x)
     if fused:
         from . import decode_ops as ops
         if st.attn_ws is None:
-            st.attn_ws = ops.attention_workspace(st.batch, d.heads, st.capacity, st.x.device)
+            st.attn_ws = (ops.attention_q8_workspace(st.q8[0], d.heads) if st.q8 else
+                          ops.attention_workspace(st.batch, d.heads, st.capacity, st.x.device))
         for i, lw in enumerate(w.layers):
-            layer_step_fused(st, lw, st.k_cache[i], st.v_cache[i], d, linear, row_linear,
-                             carry=i > 0)
+            if st.q8:
+                layer_step_fused(st, lw, None, None, d, linear, row_linear, carry=i > 0, q8=st.q8[i])
+            else:
+                layer_step_fused(st, lw, st.k_cache[i], st.v_cache[i], d, linear, row_linear,
+                                 carry=i > 0)
         ops.rmsnorm(st.x, w.final_norm, st.norm, d.eps,
                     branch=st.branch if w.layers else None)
     else:
@@ -330,13 +386,14 @@ class GraphDecoder:
     engine/engine.py:119-129: side-stream warm-up x3, then capture) and replayed per token."""
 
     def __init__(self, w: Qwen3Weights, batch: int, capacity: int, linear, device="cuda",
-                 make_hooks=None, fused=False, fused_head=False):
+                 make_hooks=None, fused=False, fused_head=False, cache="bf16"):
         """``make_hooks(state) -> (row_linear, head)`` supplies the tensor-parallel hooks,
         built once per state so their buffers are fixed before capture; ``fused`` selects the
         fused CUDA kernels for the non-linear ops; ``fused_head`` the lm_head + argmax launch
-        (no logits are stored, so ``teacher_forced_logits`` needs it off)."""
+        (no logits are stored, so ``teacher_forced_logits`` needs it off); ``cache`` "e4m3" an
+        8-bit KV cache (needs ``fused``)."""
         self.w, self.linear = w, linear
-        self.st = DecodeState(w, batch, capacity, device)
+        self.st = DecodeState(w, batch, capacity, device, cache)
         row_linear, head = make_hooks(self.st) if make_hooks else (None, None)
         if fused_head and head is None:
             head = fused_greedy_head
@@ -358,7 +415,7 @@ class GraphDecoder:
         torch.cuda.current_stream(device).wait_stream(stream)
 
     def reset(self):
-        for c in self.st.k_cache + self.st.v_cache:
+        for c in self.st.k_cache + self.st.v_cache + (self.st.q8 or []):
             c.zero_()
         self.st.position.zero_()
 

@@ -17,7 +17,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .gemm import _raise
+from .gemm import _raise, mm
 
 GROUPS = (32, 64, 128)
 _SCALE_TYPES = {torch.bfloat16: 0, torch.float16: 1}
@@ -194,3 +194,11 @@ def mm_w4(a: torch.Tensor, w: W4Weight, *, out: torch.Tensor,
     if status:
         _raise(status, f"nk_gemm_w4(M={M}, N={N}, K={K})")
     return out
+
+
+def linear(a: torch.Tensor, b, *, out: torch.Tensor) -> torch.Tensor:
+    """``out = a @ b`` for a ``W4Weight`` (``mm_w4``) or a bf16 ``W.t()`` (``mm``): the ``linear``
+    of a decode step whose layers are in 4 bits and whose lm_head is not."""
+    if isinstance(b, W4Weight):
+        return mm_w4(a, b, out=out)
+    return mm(a, b, out=out)
