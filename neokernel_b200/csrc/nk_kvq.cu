@@ -1,7 +1,6 @@
 // KV cache in 8 bits (include/nk_quant.h): the append that fills it and the attention that reads
 // it. Codes are e4m3, with one power-of-two scale per (sequence, kv head, block of tokens).
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include "nk_common.cuh"
 #include "../../include/nk_quant.h"
@@ -22,7 +21,7 @@ __device__ __forceinline__ int64_t q8_position(const int64_t* position, int per_
 // Append. RMSNorm + RoPE as qk_norm_rope_cache_kernel rounds them, a warp per 128-element head
 // row (lane l owns elements 4l .. 4l + 3; its RoPE partner is lane l ^ 16).
 //
-// A CTA of eight warps takes either eight query rows, or one (sequence, kv head, touched block):
+// A CTA of eight warps takes either eight or 32 query rows (their loads in flight together), or one (sequence, kv head, touched block):
 // it holds the block's new rows in registers (at most 16 tokens, two a warp), finds their
 // largest magnitudes, fixes the block's two scales, rounds earlier tokens' codes anew where a
 // scale rose, and stores. Each block belongs to one CTA, so nothing is shared between CTAs. A
@@ -48,26 +47,57 @@ __device__ __forceinline__ Row4 load_row4(const __nv_bfloat16* p) {
     return Row4{{bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y)}};
 }
 
+// Two floats rounded to a bf16 pair in one instruction (the low half first).
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ Row4 bf16_row(const Row4& r) {  // rounded to bf16 and back
+    const uint32_t a = bf16_pair(r.v[0], r.v[1]), b = bf16_pair(r.v[2], r.v[3]);
+    return Row4{{bf16lo(a), bf16hi(a), bf16lo(b), bf16hi(b)}};
+}
+
 // bf16 cast points of the decode step: the normalised value, its product with the gain, each
 // RoPE product, and their sum. The result's values are bf16 values.
 __device__ __forceinline__ Row4 q8_norm_rope(Row4 x, const __nv_bfloat16* gain,
                                              const __nv_bfloat16* cos_r,
                                              const __nv_bfloat16* sin_r, int lane, float eps) {
-    float ss = 0.f;
+    // The mean square and the normalised value in more than 32 bits (1 / rms as a pair of floats):
+    // an fp32 error there carries a value next to a bf16 border to the other side (one in some ten
+    // thousand), and with it an e4m3 code by a whole step. 128 elements a row: it costs 0.3 us of
+    // 2.9 at one token.
+    double ss = 0.0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ss = fmaf(x.v[i], x.v[i], ss);
-    const float inv = rsqrtf(warp_sum(ss) / (float)kHeadDim + eps);
+    for (int i = 0; i < 4; ++i) ss = fma((double)x.v[i], (double)x.v[i], ss);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+    const double inv = rsqrt(ss * (1.0 / kHeadDim) + (double)eps);
+    const float ih = (float)inv, il = (float)(inv - (double)ih);
     const Row4 w = load_row4(gain + 4 * lane), c = load_row4(cos_r + 4 * lane),
                s = load_row4(sin_r + 4 * lane);
     Row4 y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float n = bf16r(bf16r(x.v[i] * inv) * w.v[i]);
-        const float o = __shfl_xor_sync(0xffffffffu, n, 16);
-        const float rot = lane < 16 ? -o : o;
-        y.v[i] = bf16r(bf16r(n * c.v[i]) + bf16r(rot * s.v[i]));
+        const float p = x.v[i] * ih;
+        y.v[i] = p + fmaf(x.v[i], il, fmaf(x.v[i], ih, -p));
     }
-    return y;
+    y = bf16_row(y);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y.v[i] *= w.v[i];
+    y = bf16_row(y);
+    Row4 a, b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float o = __shfl_xor_sync(0xffffffffu, y.v[i], 16);
+        a.v[i] = y.v[i] * c.v[i];
+        b.v[i] = (lane < 16 ? -o : o) * s.v[i];
+    }
+    a = bf16_row(a);
+    b = bf16_row(b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a.v[i] += b.v[i];
+    return bf16_row(a);
 }
 
 // Smallest power of two s >= 2^-64 with amax <= 448 s (0 for 0). 448 = 1.75 * 2^8.
@@ -79,14 +109,15 @@ __device__ __forceinline__ float q8_scale(float amax) {
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-__device__ __forceinline__ uint32_t q8_code(float v, float inv) {  // v * inv, e4m3, NaN if not finite
-    if (!(fabsf(v) <= 3.4028235e38f)) return 0x7fu;
-    return (uint32_t)__nv_cvt_float_to_fp8(v * inv, __NV_SATFINITE, __NV_E4M3);
-}
-
-__device__ __forceinline__ uint32_t q8_codes(const Row4& r, float inv) {
-    return q8_code(r.v[0], inv) | q8_code(r.v[1], inv) << 8 | q8_code(r.v[2], inv) << 16 |
-           q8_code(r.v[3], inv) << 24;
+__device__ __forceinline__ uint32_t q8_codes(const Row4& r, float inv) {  // r * inv; NaN if not finite
+    float f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // (the conversion saturates infinities)
+        f[i] = fabsf(r.v[i]) <= 3.4028235e38f ? r.v[i] * inv : __uint_as_float(0x7fc00000u);
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(f[1]), "f"(f[0]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(f[3]), "f"(f[2]));
+    return (uint32_t)lo | (uint32_t)hi << 16;
 }
 
 __device__ __forceinline__ float2 q8_decode2(uint32_t codes16) {
@@ -112,6 +143,8 @@ __device__ __forceinline__ float finite_max(const Row4& r, float m) {
 
 constexpr int kQ8Warps = 8;
 
+// QR: query rows per warp.
+template <int QR>
 __global__ void __launch_bounds__(32 * kQ8Warps) q8_append_kernel(const Q8AppendArgs a) {
     __shared__ float s_max[2][kQ8Warps];
     if (threadIdx.x == 0) griddep_launch_dependents();
@@ -126,16 +159,25 @@ __global__ void __launch_bounds__(32 * kQ8Warps) q8_append_kernel(const Q8Append
     }
     const int T = a.tokens;
     if ((int)blockIdx.x < a.q_ctas) {  // query rows
-        const int row = blockIdx.x * kQ8Warps + warp;
-        if (row >= T * a.hq) return;
-        const int t = row / a.hq, h = row - t * a.hq;
-        const Row4 x = load_row4(a.qkv + ((int64_t)b * T + t) * a.ld + h * kHeadDim + 4 * lane);
-        const Row4 y = q8_norm_rope(x, a.qn, a.cos_t + (pos + t) * kHeadDim,
-                                    a.sin_t + (pos + t) * kHeadDim, lane, a.eps);
-        uint2 o;
-        o.x = pack_bf16x2(y.v[0], y.v[1]);
-        o.y = pack_bf16x2(y.v[2], y.v[3]);
-        *reinterpret_cast<uint2*>(a.q_out + (((int64_t)b * T + t) * a.hq + h) * kHeadDim + 4 * lane) = o;
+        const int row0 = (blockIdx.x * kQ8Warps + warp) * QR, rows = T * a.hq;
+        const __nv_bfloat16* base = a.qkv + (int64_t)b * T * a.ld + 4 * lane;
+        __nv_bfloat16* out = a.q_out + ((int64_t)b * rows) * kHeadDim + 4 * lane;
+        Row4 x[QR];
+        int t[QR];
+#pragma unroll
+        for (int i = 0; i < QR; ++i) {
+            const int row = min(row0 + i, rows - 1);
+            t[i] = row / a.hq;
+            x[i] = load_row4(base + t[i] * a.ld + (row - t[i] * a.hq) * kHeadDim);
+        }
+#pragma unroll
+        for (int i = 0; i < QR; ++i) {
+            const Row4 y = q8_norm_rope(x[i], a.qn, a.cos_t + (pos + t[i]) * kHeadDim,
+                                        a.sin_t + (pos + t[i]) * kHeadDim, lane, a.eps);
+            if (row0 + i < rows)
+                *reinterpret_cast<uint2*>(out + (int64_t)(row0 + i) * kHeadDim) =
+                    make_uint2(bf16_pair(y.v[0], y.v[1]), bf16_pair(y.v[2], y.v[3]));
+        }
         return;
     }
     const int u = blockIdx.x - a.q_ctas;
@@ -701,7 +743,7 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 const float f = (Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift)) / L;
                 *reinterpret_cast<uint2*>(
                     a.out + (((int64_t)b * a.tokens + tok) * a.hq + (int64_t)h * a.G + hh) * kHeadDim +
-                    4 * lane) = make_uint2(pack_bf16x2(A.x * f, A.y * f), pack_bf16x2(A.z * f, A.w * f));
+                    4 * lane) = make_uint2(bf16_pair(A.x * f, A.y * f), bf16_pair(A.z * f, A.w * f));
             } else {
                 float* p = part + r * kQ8PartFloats;
                 *reinterpret_cast<float4*>(p + 4 * lane) = A;
@@ -808,7 +850,7 @@ __global__ void __launch_bounds__(32 * kQ8MergeWarps) q8_merge_kernel(const Q8At
     }
     if (!shared_pair) return;
     const float f = (Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift)) / L;
-    *out = make_uint2(pack_bf16x2(A.x * f, A.y * f), pack_bf16x2(A.z * f, A.w * f));
+    *out = make_uint2(bf16_pair(A.x * f, A.y * f), bf16_pair(A.z * f, A.w * f));
 }
 
 static bool q8_heads_ok(int tokens, int hq, int hkv) {
@@ -912,10 +954,15 @@ extern "C" int nk_qk_norm_rope_cache_q8(const void* qkv, int64_t ld_qkv, const v
     a.ch = c->head_stride;
     a.cs = c->seq_stride;
     a.eps = eps;
-    a.q_ctas = (tokens * q_heads + kQ8Warps - 1) / kQ8Warps;
     const int touched = (tokens + c->block - 2) / c->block + 1;  // blocks that T tokens can touch
-    return launch_pdl_smem(q8_append_kernel, dim3(a.q_ctas + c->kv_heads * touched, c->batch),
-                           dim3(32 * kQ8Warps), 0, (cudaStream_t)stream, a);
+    // One query row per warp while that fits the GPU at once (eight CTAs per SM), four beyond:
+    // measured at 16 sequences x 16 tokens x 64 heads, see the figures above.
+    const bool many = (int64_t)c->batch * tokens * q_heads > 8ll * kNumSMs * kQ8Warps;
+    const int per_cta = kQ8Warps * (many ? 4 : 1);
+    a.q_ctas = (tokens * q_heads + per_cta - 1) / per_cta;
+    const dim3 grid(a.q_ctas + c->kv_heads * touched, c->batch), block(32 * kQ8Warps);
+    return many ? launch_pdl_smem(q8_append_kernel<4>, grid, block, 0, (cudaStream_t)stream, a)
+                : launch_pdl_smem(q8_append_kernel<1>, grid, block, 0, (cudaStream_t)stream, a);
 }
 
 extern "C" size_t nk_attention_q8_ws_bytes(int tokens, int q_heads, int kv_heads) {
