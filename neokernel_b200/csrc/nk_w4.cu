@@ -469,28 +469,33 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
         bool ok = true;
         int st = set, wph = 0, xs = XS - 2 + set, xph = 1;  // xs, xph: of step i - 2
         int ready = set;
-#pragma unroll 1
-        for (int i = set; i < n; i += SETS) {
-            const uint32_t ab = i & 1;
+        uint4 u[4];         // the step's codes of this row, and its groups' zero points: fetched
+        uint32_t zc[NG];    // before the step before it is handed over
+        auto fetch = [&]() {
             ok = __all_sync(0xffffffffu, w4_wait(bar_full + 8 * st, wph));
-            if (!ok) break;
-            const uint32_t w = base + L::kWOff + st * L::kW;
-            uint32_t zc[NG];
+            if (!ok) return;
+            const uint32_t w = L::kWOff + st * L::kW;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) u[c] = lds128(base + w + c * 2048 + row * 16);
 #pragma unroll
             for (int j = 0; j < NG; ++j)
-                zc[j] = ZP ? w4_zero(gbase[L::kWOff + st * L::kW + kW4StepBytes + L::kScale +
-                                           j * kW4Rows + row])
+                zc[j] = ZP ? w4_zero(gbase[w + kW4StepBytes + L::kScale + j * kW4Rows + row])
                            : 0xbe00be00u;
-            uint4 u[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) u[c] = lds128(w + c * 2048 + row * 16);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_empty + 8 * st);
+            if ((st += SETS) >= WS) {
+                st -= WS;
+                wph ^= 1;
+            }
+        };
+        if (set < n) fetch();
+#pragma unroll 1
+        for (int i = set; i < n && ok; i += SETS) {
             // the MMAs of step i - 2 have read this buffer (passes at once for the first two)
             ok = __all_sync(0xffffffffu, w4_wait(bar_done + 8 * xs, xph));
             if (!ok) break;
             tc_fence_after();
-            const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16) + ab * 64;
+            const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16) + (i & 1) * 64;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {  // 32 K elements: one group or part of one
                 const uint32_t z = zc[c * NG / 4];
@@ -505,15 +510,12 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
                 }
                 tmem_st16(ta + c * 16, r);
             }
+            if (i + SETS < n) fetch();
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_ready + 8 * ready);
             if ((ready += SETS) >= XS) ready -= XS;
-            if ((st += SETS) >= WS) {
-                st -= WS;
-                wph ^= 1;
-            }
             if ((xs += SETS) >= XS) {
                 xs -= XS;
                 xph ^= 1;
@@ -569,35 +571,26 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
     cluster_wait();
 }
 
-#ifdef W4_TUNE
-extern "C" { __attribute__((visibility("default"))) int w4_tune_s = 0; }
-#endif
-
 template <int NT, int NG, bool ZP, bool FP16>
 static int w4_launch(const W4Args& a, cudaStream_t s) {
     using L = W4Smem<NT, NG>;
     auto kernel = w4_kernel<NT, NG, ZP, FP16>;
-    static int sms[64] = {};  // multiprocessors, once the kernel's shared-memory limit is raised
+    static bool ready[64] = {};  // per device: the kernel's shared-memory limit is raised
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return NK_ERR_CUDA;
     if (dev < 0 || dev >= 64) return NK_ERR_DEVICE;
-    if (sms[dev] == 0) {
-        int n = 0;
+    if (!ready[dev]) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc) !=
                 cudaSuccess ||
             cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                 (int)cudaSharedmemCarveoutMaxShared) != cudaSuccess ||
-            cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+                                 (int)cudaSharedmemCarveoutMaxShared) != cudaSuccess)
             return NK_ERR_CUDA;
-        sms[dev] = n;
+        ready[dev] = true;
     }
     const int tiles = (a.N + kW4Rows - 1) / kW4Rows, mt = (a.M + NT - 1) / NT;
     // K is split while the CTAs still fit the GPU at once and keep two steps each
     int S = (int)min((int64_t)kW4MaxCluster, (int64_t)256 / ((int64_t)tiles * mt));
     S = max(1, min(S, a.KB / 2));
-#ifdef W4_TUNE
-    if (w4_tune_s) S = min(w4_tune_s, a.KB);
-#endif
     CUtensorMap mx{};
     if (a.wide_x && (get_encoder() != NK_OK || make_map(&mx, a.x, a.M, a.K, a.ldx, NT) != NK_OK))
         return NK_ERR_CUDA;
