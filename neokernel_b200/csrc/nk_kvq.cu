@@ -21,11 +21,13 @@ __device__ __forceinline__ int64_t q8_position(const int64_t* position, int per_
 // Append. RMSNorm + RoPE as qk_norm_rope_cache_kernel rounds them, a warp per 128-element head
 // row (lane l owns elements 4l .. 4l + 3; its RoPE partner is lane l ^ 16).
 //
-// A CTA of eight warps takes either eight or 32 query rows (their loads in flight together), or one (sequence, kv head, touched block):
-// it holds the block's new rows in registers (at most 16 tokens, two a warp), finds their
+// A CTA of eight warps takes either query rows (one or four a warp, their loads in flight
+// together), or one (sequence, kv head, touched block): it holds the block's new rows in registers (at most 16 tokens, two a warp), finds their
 // largest magnitudes, fixes the block's two scales, rounds earlier tokens' codes anew where a
 // scale rose, and stores. Each block belongs to one CTA, so nothing is shared between CTAs. A
-// few hundred KB move at most; the launch and two dependent round trips to memory bound it.
+// few hundred KB move at most; the launch and two dependent round trips to memory bound it (2.8 us
+// at one token, of which an empty launch in a row of launches is 1.7; 7.5 us, 1.4 TB/s, at 16
+// sequences of 16 tokens and 64 heads).
 // ---------------------------------------------------------------------------------------
 struct Q8AppendArgs {
     const __nv_bfloat16* qkv; int64_t ld;
@@ -529,7 +531,7 @@ q8_attn_kernel(const Q8AttnArgs a) {
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
             // largest magnitude to [2^12, 2^13): a bf16 value keeps its 8 bits down to 2^-29 of it
             int e = (int)(__float_as_uint(m) >> 23) - 127 - 12;
-            e = min(max(e, -100), 100);
+            e = min(max(e, -100), 115);
             const float up = __uint_as_float((uint32_t)(127 - e) << 23);
             const float down = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
@@ -610,7 +612,7 @@ q8_attn_kernel(const Q8AttnArgs a) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[nt][e] *= qs[nt][e & 1] * k_scale;
+                    for (int e = 0; e < 4; ++e) s[nt][e] = s[nt][e] * k_scale * qs[nt][e & 1];
                     if (!all_seen) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
@@ -665,6 +667,43 @@ q8_attn_kernel(const Q8AttnArgs a) {
                     }
                     pf[nt][0] = movm_t(pack_f16x2(f[0][0], f[0][1]));
                     pf[nt][1] = movm_t(pack_f16x2(f[1][0], f[1][1]));
+                }
+                // A NaN among new tokens' values must not reach the rows before it (0 * NaN): it is
+                // made 0 here and given to the sums of the rows that see it. Byte i of `first`: first
+                // slot of the tile with one in element 4 lane + i, 0xff for none.
+                if (!all_seen && a.tokens > 1) {
+                    const uint32_t v0 = ring + stage * kQ8WarpStage + 16 * 128 + (lane & 3) * 4;
+                    uint32_t first = 0xffffffffu;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const uint32_t at = v0 + j * 128 + (((lane >> 2) ^ (j & 7)) << 4);
+                        uint32_t w;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+                        const uint32_t bad = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                        if (bad) {
+                            const uint32_t bytes = (bad >> 7) * 0xffu;
+                            const uint32_t open = ((first >> 7) & 0x01010101u) * 0xffu & bytes;
+                            first = (first & ~open) | (j * 0x01010101u & open);
+                            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w & ~bytes) : "memory");
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, first != 0xffffffffu)) {
+#pragma unroll
+                        for (int d = 0; d < 8; ++d) {
+                            const uint32_t w = __shfl_sync(0xffffffffu, first, 4 * d + (g >> 1)) >> (16 * (g & 1));
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const int j = (w >> (8 * k)) & 0xff;
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                    for (int i = 0; i < 2; ++i)
+                                        if (j < 16 && j0 + j - pos <= last[nt][i])
+                                            o[d][nt][i + 2 * k] = __uint_as_float(0x7fc00000u);
+                            }
+                        }
+                    }
+                    __syncwarp();
                 }
                 // V^T: rows of tile d are dims 16 d + 2 g (first eight) and 16 d + 2 g + 1
 #pragma unroll
@@ -955,9 +994,9 @@ extern "C" int nk_qk_norm_rope_cache_q8(const void* qkv, int64_t ld_qkv, const v
     a.cs = c->seq_stride;
     a.eps = eps;
     const int touched = (tokens + c->block - 2) / c->block + 1;  // blocks that T tokens can touch
-    // One query row per warp while that fits the GPU at once (eight CTAs per SM), four beyond:
-    // measured at 16 sequences x 16 tokens x 64 heads, see the figures above.
-    const bool many = (int64_t)c->batch * tokens * q_heads > 8ll * kNumSMs * kQ8Warps;
+    // One query row per warp while that is at most five CTAs per SM, four rows beyond: measured
+    // (one a warp / four) 4.2 / 5.1 us at 4096 query rows, 6.3 / 6.0 at 8192, 8.6 / 7.5 at 16384.
+    const bool many = (int64_t)c->batch * tokens * q_heads > 5ll * kNumSMs * kQ8Warps;
     const int per_cta = kQ8Warps * (many ? 4 : 1);
     a.q_ctas = (tokens * q_heads + per_cta - 1) / per_cta;
     const dim3 grid(a.q_ctas + c->kv_heads * touched, c->batch), block(32 * kQ8Warps);

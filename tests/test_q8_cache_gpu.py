@@ -193,6 +193,39 @@ def test_attention_nan_is_not_lost(where):
         assert torch.equal(row[:2, :7], before[:2, :7])
 
 
+@pytest.mark.parametrize("T,heads,kv", [(4, 4, 2), (16, 4, 2), (5, 8, 1), (2, 16, 1)])
+@pytest.mark.parametrize("pos", (0, 13, 250))
+def test_attention_nan_in_later_tokens_stays_there(T, heads, kv, pos):
+    """A draft token whose value or key is not finite: the rows before it do not see it."""
+    cache = filled_cache(1, kv, 300, 64, seed=11)
+    q = rand(T, heads * 128, seed=12)
+    clean = run_attention(q, cache, [pos], heads).view(T, heads, 128)
+    v = cache.v.view(torch.uint8)
+    v[0, 0, pos + T - 1, 7] = 0x7f
+    v[0, 0, pos + T // 2, 40:100] = 0xff
+    out = run_attention(q, cache, [pos], heads).view(T, heads, 128)
+    want = clean.clone()
+    G = heads // kv
+    want[T - 1:, :G, 7] = float("nan")
+    want[T // 2:, :G, 40:100] = float("nan")
+    same = (out == want) | (out.isnan() & want.isnan())
+    assert same.all()
+    cache.k.view(torch.uint8)[0, 0, pos + T - 1, 3] = 0x7f
+    out = run_attention(q, cache, [pos], heads).view(T, heads, 128)
+    want[T - 1:, :G] = float("nan")
+    assert ((out == want) | (out.isnan() & want.isnan())).all()
+
+
+def test_attention_queries_next_to_the_largest():
+    """Scores of 0 whatever the query's size: the mean of the values."""
+    cache = filled_cache(1, 1, 128, 64, seed=8)
+    cache.k_scale.zero_()
+    q = torch.full((1, 128), torch.finfo(torch.bfloat16).max, dtype=torch.bfloat16, device=DEV)
+    check_attention(q, cache, [127], 1)
+    cache.k_scale.fill_(2.0 ** -64)
+    check_attention(q * 2.0 ** -66, cache, [127], 1)
+
+
 def test_attention_large_and_tiny_queries():
     cache = filled_cache(1, 1, 128, 64, seed=8)
     for std in (1e-30, 1e-4, 30.0):
