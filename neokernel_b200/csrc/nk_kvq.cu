@@ -25,9 +25,9 @@ __device__ __forceinline__ int64_t q8_position(const int64_t* position, int per_
 // together), or one (sequence, kv head, touched block): it holds the block's new rows in registers (at most 16 tokens, two a warp), finds their
 // largest magnitudes, fixes the block's two scales, rounds earlier tokens' codes anew where a
 // scale rose, and stores. Each block belongs to one CTA, so nothing is shared between CTAs. A
-// few hundred KB move at most; the launch and two dependent round trips to memory bound it (2.8 us
-// at one token, of which an empty launch in a row of launches is 1.7; 7.5 us, 1.4 TB/s, at 16
-// sequences of 16 tokens and 64 heads).
+// few hundred KB move at most; the launch and two dependent round trips to memory bound it (2.7 us
+// at one token, 0.75 where every sequence is idle; 7.5 us at 16 sequences of 16 tokens and 64
+// heads, 1.3 TB/s).
 // ---------------------------------------------------------------------------------------
 struct Q8AppendArgs {
     const __nv_bfloat16* qkv; int64_t ld;
@@ -281,8 +281,14 @@ __global__ void __launch_bounds__(32 * kQ8Warps) q8_append_kernel(const Q8Append
 // A pair covered by one CTA is written directly; otherwise its CTAs write (m, my, l, O) of their
 // part, and a second launch adds the parts in order of their slots, its rows spread over the
 // GPU. (Measured: the last CTA of a pair adding the parts in the first launch instead takes
-// 11.2 us where the two launches take 8.5, at one sequence of 1024 slots, and 60 where they take
+// 11.2 us where the two launches took 8.5, at one sequence of 1024 slots, and 60 where they took
 // 30 at five of 3000 with 32 query rows: one CTA walks through all rows of the pair.)
+//
+// Measured, 8 kv heads (us, both launches; in brackets the cache's bytes at 6456 GB/s): two
+// sequences of 128k slots 86.4 [83.2], 6.2 TB/s; 16 ragged ones of up to 8192 slots 32.6 [22.0]; one
+// of 1024 slots 7.5 [0.3]; five of up to 3000, four tokens x 64 heads, 20.4 [2.8]. Long caches
+// stream at the copy rate; the fixed part (two launches, first bytes, join) is some 7 us; many
+// query rows are bound by the conversions and the matrix instructions (issue slots 45% busy).
 // ---------------------------------------------------------------------------------------
 constexpr int kQ8Unit = 64;                 // slots per unit, 16 per warp
 constexpr int kQ8AttnThreads = 128;

@@ -14,6 +14,18 @@
 // take the widened weights (four times the stream again), tensor memory can: the weights are the
 // MMA's A operand there (128 rows = 128 lanes), the tokens its B operand in shared memory.
 //
+// Measured in CUDA graphs (us; in brackets the weight bytes' time at 6456 GB/s, the copy rate):
+//   N 24576, K 4096   M=1 16.1 [8.0], M=64 26.4 [8.3]     group 128
+//   N 6144, K 4096    M=16 8.0 [2.1]                      group 64
+//   N 4096, K 12288   M=8 12.9 [4.7]                      group 32 with zero points
+//   N 1024, K 2048    M=1 3.4 [0.2]: the launch and one pass through the pipeline
+// Per step of 128 x 128 the eight MMAs take some 256 cycles (each reads 4 KB of A from tensor
+// memory at 128 bytes a cycle), and a step of a CTA 450 to 500, with its barriers. So what bounds
+// the wide shapes is the time per step on the SMs that hold two CTAs while others hold one (192
+// row tiles on 148 SMs), the narrow ones the fixed parts (some 3 us: launch, first bytes, the
+// cluster's sum). On mma.sync, with the weights widened in registers, the same cases took 14.2
+// (M=1), 75 (M=64), 12 and 19 us.
+//
 // A CTA takes 128 weight rows and a range of K steps (128 wide). Its warps:
 //   0      lane 0 streams codes, scales and zero points of each step (one contiguous 8 KB piece
 //          and two small ones) through a ring of bulk copies
@@ -588,7 +600,10 @@ static int w4_launch(const W4Args& a, cudaStream_t s) {
         ready[dev] = true;
     }
     const int tiles = (a.N + kW4Rows - 1) / kW4Rows, mt = (a.M + NT - 1) / NT;
-    // K is split while the CTAs still fit the GPU at once and keep two steps each
+    // K is split while the CTAs still fit the GPU at once (clusters of up to eight pack into its
+    // GPCs up to some 256 CTAs, two an SM; more wait for a second wave) and keep two steps each.
+    // Measured: 48 tiles, S = 4 / 5 / 6 / 8 (288 and 384 CTAs): 7.9 / 8.1 / 12.6 / 11.6 us; 32 tiles,
+    // S = 5 / 7 / 8: 16.1 / 13.6 / 12.7; 192 tiles, S = 1 / 2 / 3: 16.5 / 18.4 / 23.7.
     int S = (int)min((int64_t)kW4MaxCluster, (int64_t)256 / ((int64_t)tiles * mt));
     S = max(1, min(S, a.KB / 2));
     CUtensorMap mx{};
@@ -674,6 +689,9 @@ extern "C" int nk_gemm_w4(const void* x, int64_t ldx, const nk_w4_weight* w, voi
     a.wide_x = ((uintptr_t)x & 15u) == 0 && a.ldx % 8 == 0;
     const bool fp16 = w->scale_type == NK_W4_SCALE_FP16;
     cudaStream_t s = (cudaStream_t)stream;
+    // the narrowest token tile that holds M (a wider one costs MMA columns, fold registers and ring
+    // stages: N 24576, K 4096 takes 16.1 us with 16 columns, 26.4 with 64); beyond 64 tokens the
+    // weights are read once per 64
     if (M <= 16) return w4_dispatch<16>(a, group, fp16, s);
     if (M <= 32) return w4_dispatch<32>(a, group, fp16, s);
     return w4_dispatch<64>(a, group, fp16, s);
