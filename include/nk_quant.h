@@ -53,7 +53,7 @@ NK_API size_t nk_w4_scale_bytes(int N, int K, int group);
 NK_API size_t nk_w4_zero_bytes(int N, int K, int group);
 
 /* x: [M, K] bf16, row stride ldx >= K (elements); y: [M, N] bf16, row stride ldy >= N; both 2-byte
- * aligned (x 16-byte aligned with ldx % 8 == 0 is read by TMA). Any M from 1 to 2^20. No
+ * aligned (x 16-byte aligned with ldx % 8 == 0 is read by TMA); y not in x's memory. Any M from 1 to 2^20. No
  * workspace. The weights must have been written before the launch that precedes this one on the
  * stream (they are read ahead of it); weights made at load time always are. */
 NK_API int nk_gemm_w4(const void* x, int64_t ldx, const nk_w4_weight* w, void* y, int64_t ldy,
@@ -63,9 +63,9 @@ NK_API int nk_gemm_w4(const void* x, int64_t ldx, const nk_w4_weight* w, void* y
  *
  * Keys and values are e4m3 codes (1 byte, finite range +-448) times a scale held for each
  * (sequence, kv head, block of `block` token slots), in fp32 [batch][kv_heads][ceil(capacity /
- * block)]. block is 16, 32, 64 or 128. Code arrays have unit stride along the 128 head
- * elements and any batch, head and token strides that are multiples of 16 (bytes).
- * capacity <= 2^30.
+ * block)]. block is 16, 32, 64 or 128. Code arrays have unit stride along the 128 head elements
+ * and any batch, head and token strides that are multiples of 16 (bytes); no two sequences,
+ * heads, tokens or arrays share memory. capacity <= 2^30.
  *
  * `position` is a device int64 array: entry b (or entry 0 for every sequence when
  * per_sequence == 0) is the slot of sequence b's first new token; `tokens` (1..16) new tokens take
@@ -101,7 +101,8 @@ typedef struct nk_q8_cache {
  * that is not finite. Slots past the new tokens, and everything of an idle sequence (its q_out
  * rows included), are left as they are.
  *   qkv: [batch * tokens, (q_heads + 2 kv_heads) * 128] bf16, row stride ld_qkv, row b * tokens + t
- *   q_out: [batch * tokens, q_heads * 128] bf16; q_norm, k_norm: [128]; cos, sin: [capacity, 128]
+ *   q_out: [batch * tokens, q_heads * 128] bf16, not in qkv's memory
+ *   q_norm, k_norm: [128]; cos, sin: [capacity, 128]
  * bf16 pointers 8-byte aligned and ld_qkv a multiple of 4. */
 NK_API int nk_qk_norm_rope_cache_q8(const void* qkv, int64_t ld_qkv, const void* q_norm,
                                     const void* k_norm, const void* cos_table,

@@ -179,6 +179,7 @@ class Q8Cache:
                   "capacity, 128]")
         _need(v.shape == k.shape and v.stride() == k.stride() and v.device == k.device,
               "Q8Cache: k and v must have the same shape, strides and device")
+        _need(v.data_ptr() != k.data_ptr(), "Q8Cache: k and v must not share memory")
         _need(block in Q8_BLOCKS, f"Q8Cache: block must be one of {Q8_BLOCKS}, got {block}")
         B, H, S, _ = k.shape
         _need(1 <= B <= Q8_MAX_BATCH and H >= 1 and S >= 1,
@@ -197,6 +198,8 @@ class Q8Cache:
             _need(isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.device == k.device
                   and tuple(t.shape) == shape and t.is_contiguous(),
                   f"Q8Cache: scales must be contiguous fp32 {list(shape)} on the codes' device")
+        _need(k_scale.data_ptr() != v_scale.data_ptr(),
+              "Q8Cache: k_scale and v_scale must not share memory")
         self.k, self.v, self.k_scale, self.v_scale, self.block = k, v, k_scale, v_scale, block
         self.batch, self.kv_heads, self.capacity, self.device = B, H, S, k.device
         self._c = _lib.NkQ8Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
@@ -283,7 +286,8 @@ def qk_norm_rope_cache_q8(qkv, q_norm, k_norm, cos, sin, position, q_out, cache:
 
     qkv [batch * T, (heads + 2 kv_heads) * 128] (row b * T + t, unit column stride); ``position``
     [batch] (or [1], shared): slot of each sequence's first new token, negative for an idle
-    sequence, of which nothing is read or written. q_out [batch * T, heads * 128] contiguous. A
+    sequence, of which nothing is read or written. q_out [batch * T, heads * 128] contiguous, not
+    in qkv's memory. A
     block's scale is the smallest power of two that keeps its new tokens within e4m3's range,
     and at least its former one where it holds earlier tokens; these are rounded anew when it
     rises. A position past capacity - T is an idle sequence too and is reported by

@@ -118,6 +118,8 @@ class W4Weight:
             s = (w.abs().amax(-1) / 7.0).to(scale_dtype)
             sf = torch.where(s > 0, s.float(), torch.ones_like(w[..., 0]))
             z = torch.full_like(sf, 8.0)
+        _need(bool(s.isfinite().all()), "W4Weight: weight must be finite, and its groups' scales "
+              f"within {scale_dtype}")
         q = (torch.round(w / sf[..., None]) + z[..., None]).clamp(0, 15).to(torch.uint8)
         q = q.view(N, -1)[:, :K]
         if K % 2:
@@ -154,7 +156,8 @@ def mm_w4(a: torch.Tensor, w: W4Weight, *, out: torch.Tensor,
           stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """``out = a @ W.t()`` for a 4-bit weight ``w`` of W [N, K]: fp32 sums, one bf16 rounding.
 
-    a: bf16 CUDA [M, K] with unit column stride; out: bf16 CUDA [M, N] with unit column stride.
+    a: bf16 CUDA [M, K] with unit column stride; out: bf16 CUDA [M, N] with unit column stride, in
+    memory that ``a`` does not share.
     Any M; made for decode batches and drafts of up to 64 tokens (larger ones read the weights once
     per 64 tokens).
     """

@@ -469,3 +469,13 @@ def test_refusals():
                  (k, cache.v, s, s, 32)):
         with pytest.raises(ValueError):
             ops.Q8Cache(*args)
+
+
+def test_cache_refuses_shared_arrays():
+    c = ops.Q8Cache.empty(1, 2, 64, DEV)
+    with pytest.raises(ValueError, match="share"):
+        ops.Q8Cache(c.k, c.k, c.k_scale, c.v_scale, 64)
+    with pytest.raises(ValueError, match="share"):
+        ops.Q8Cache(c.k, c.v, c.k_scale, c.k_scale, 64)
+    both = torch.zeros(1, 2, 64, 2, 128, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    ops.Q8Cache(both[..., 0, :], both[..., 1, :], c.k_scale, c.v_scale, 64)  # side by side

@@ -193,3 +193,16 @@ def test_q8_cache_refuses_cpu_tensors_and_bad_blocks():
         ops.Q8Cache.empty(1, 2, 64, "cpu", block=24)
     with pytest.raises(ValueError):
         ops.Q8Cache.empty(1, 2, 64, "cpu", layout="sbhd")
+
+
+def test_quantize_refuses_what_has_no_scale():
+    for bad in (float("nan"), float("inf")):
+        w = torch.ones(4, 64)
+        w[2, 5] = bad
+        for zeros in (False, True):
+            with pytest.raises(ValueError, match="finite"):
+                nk.W4Weight.quantize(w, 32, zeros=zeros)
+    w = torch.full((2, 32), 1e6)  # 1e6 / 7 is past fp16
+    with pytest.raises(ValueError, match="finite"):
+        nk.W4Weight.quantize(w, 32, scale_dtype=torch.float16)
+    assert torch.isfinite(nk.W4Weight.quantize(w, 32).dequantize()).all()
