@@ -278,6 +278,9 @@ __global__ void __launch_bounds__(32 * kQ8Warps) q8_append_kernel(const Q8Append
 // to f16 (11 bits, from 2^15 down to 2^-24: what underflows is below 2^-39 of the largest
 // term), while the sum l = sum 2^(x - m) stays in fp32. Then out = (O / l) 2^(my - m).
 //
+// Short caches take the same walk in another frame: a cluster of CTAs per pair, joined through
+// distributed shared memory in one launch (the rule and its figures are in nk_attention_decode_q8).
+//
 // A pair covered by one CTA is written directly; otherwise its CTAs write (m, my, l, O) of their
 // part, and a second launch adds the parts in order of their slots, its rows spread over the
 // GPU. (Measured: the last CTA of a pair adding the parts in the first launch instead takes
@@ -286,8 +289,8 @@ __global__ void __launch_bounds__(32 * kQ8Warps) q8_append_kernel(const Q8Append
 //
 // Measured, 8 kv heads (us, both launches; in brackets the cache's bytes at 6456 GB/s): two
 // sequences of 128k slots 86.4 [83.2], 6.2 TB/s; 16 ragged ones of up to 8192 slots 32.6 [22.0]; one
-// of 1024 slots 7.5 [0.3]; five of up to 3000, four tokens x 64 heads, 20.4 [2.8]. Long caches
-// stream at the copy rate; the fixed part (two launches, first bytes, join) is some 7 us; many
+// of 1024 slots (a cluster per pair) 5.0 [0.3]; five of up to 3000, four tokens x 64 heads, 20.4 [2.8]. Long caches
+// stream at the copy rate; the fixed part (first bytes, join; two launches) is some 4 to 7 us; many
 // query rows are bound by the conversions and the matrix instructions (issue slots 45% busy).
 // ---------------------------------------------------------------------------------------
 constexpr int kQ8Unit = 64;                 // slots per unit, 16 per warp
@@ -307,6 +310,16 @@ constexpr int kQ8MaxGrid = 148 * 4;
 constexpr int kQ8PartFloats = kHeadDim + 4; // O, then m, my, l
 constexpr float kQ8Shift = 15.f;            // probabilities are held times 2^15
 constexpr int kQ8MergeWarps = 8;
+constexpr int kQ8MaxCluster = 8;
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t saddr, uint32_t rank) {
+    uint32_t a;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
 
 struct Q8AttnArgs {
     const __nv_bfloat16* q;
@@ -319,6 +332,7 @@ struct Q8AttnArgs {
     int rows, row_blocks;        // query rows of a CTA (8 NT), row blocks of a pair's T * G rows
     int grid;                    // CTAs of the first launch
     int lg_wpr;                  // merge: log2 of the warps that share a row
+    int lg_cluster;              // short-cache form: log2 of the cluster's CTAs
     int64_t cb, ch, cs;
     float scale_log2;            // softmax scale times log2(e)
 };
@@ -390,11 +404,13 @@ struct Q8Split {
     }
 };
 
-template <int NT>
+// CL: the short-cache form. A cluster of 2, 4 or 8 CTAs shares one pair's units and joins through
+// distributed shared memory: no partition over pairs, no partial sums in memory, no second launch.
+template <int NT, bool CL>
 __global__ void __launch_bounds__(kQ8AttnThreads, 3)
 q8_attn_kernel(const Q8AttnArgs a) {
     extern __shared__ __align__(1024) uint8_t q8_smem[];
-    __shared__ int s_end[NK_Q8_MAX_BATCH];              // running sum of the sequences' units
+    __shared__ int s_end[CL ? 1 : NK_Q8_MAX_BATCH];     // running sum of the sequences' units
     __shared__ float s_stat[4][8 * NT][4];
     __shared__ uint2 s_q[NT > 1 ? NT * 8 * 32 : 1];     // Q^T operand, shared by the warps
     __shared__ float s_down[8 * NT];                    // and its rows' powers of two
@@ -402,7 +418,10 @@ q8_attn_kernel(const Q8AttnArgs a) {
     griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    if (warp == 0) {  // 128 sequences at a time, their positions read together
+    const uint32_t per_b = a.hkv * a.row_blocks;        // pairs per sequence
+    const int total_rows = a.tokens * a.G;
+    uint32_t u = 0, u_end = 0, G = 0, U = 0;
+    if (!CL && warp == 0) {  // 128 sequences at a time, their positions read together
         int base = 0;
         for (int b0 = 0; b0 < a.batch; b0 += 128) {
             int x[4];
@@ -430,38 +449,58 @@ q8_attn_kernel(const Q8AttnArgs a) {
             if (a.position[a.per_sequence ? b : 0] > (int64_t)a.capacity - a.tokens)
                 atomicExch(&g_error, NK_ERR_RANGE);
     }
-    __syncthreads();
-    const uint32_t per_b = a.hkv * a.row_blocks;            // pairs per sequence
-    const uint32_t U = s_end[a.batch - 1] * per_b;
-    const uint32_t G = min((uint32_t)a.grid, U);            // no CTA of the partition is empty
-    const int total_rows = a.tokens * a.G;
+    if (!CL) {
+        __syncthreads();
+        U = s_end[a.batch - 1] * per_b;
+        G = min((uint32_t)a.grid, U);                   // no CTA of the partition is empty
+    }
     // rows of idle sequences are zero
-    for (int b = blockIdx.x; b < a.batch; b += a.grid)
-        if (s_end[b] == (b > 0 ? s_end[b - 1] : 0)) {
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
+        if (CL ? q8_seq_units(a, b) == 0 : s_end[b] == (b > 0 ? s_end[b - 1] : 0)) {
             const int vecs = a.tokens * a.hq * (kHeadDim / 4);
             uint2* o = reinterpret_cast<uint2*>(a.out + (int64_t)b * a.tokens * a.hq * kHeadDim);
             for (int i = threadIdx.x; i < vecs; i += kQ8AttnThreads) o[i] = make_uint2(0u, 0u);
         }
-    if (blockIdx.x >= G) return;
-    const Q8Split split(U, G);
-    uint32_t u = split.begin(blockIdx.x);
-    const uint32_t u_end = split.begin(blockIdx.x + 1);
+    if (!CL) {
+        if (blockIdx.x >= G) return;
+        const Q8Split split(U, G);
+        u = split.begin(blockIdx.x);
+        u_end = split.begin(blockIdx.x + 1);
+    }
     const uint32_t smem0 = static_cast<uint32_t>(__cvta_generic_to_shared(q8_smem));
     const uint32_t ring = smem0 + warp * (kQ8Stages * kQ8WarpStage);
     const uint32_t s_scale = smem0 + q8_scale_off(NT) + warp * (kQ8Stages * 8);
 
-    while (u < u_end) {
-        // the pair of unit u: sequence b, kv head h, row block rb; its units [p0, p0 + n)
-        int lo = 0, hi = a.batch - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (s_end[mid] * per_b > u) hi = mid; else lo = mid + 1;
+    do {
+        // the pair of unit u: sequence b, kv head h, row block rb; its units [p0, p0 + n), of which
+        // this CTA takes [c0, c1)
+        int b, c0, c1;
+        uint32_t n, pr, p0 = 0;
+        if (CL) {
+            const uint32_t pair = blockIdx.x >> a.lg_cluster;
+            const uint32_t rank = blockIdx.x - (pair << a.lg_cluster);
+            b = pair / per_b;
+            pr = pair - b * per_b;
+            n = q8_seq_units(a, b);
+            if (n == 0) return;  // (the whole cluster)
+            c0 = n * rank >> a.lg_cluster;
+            c1 = n * (rank + 1) >> a.lg_cluster;
+        } else {
+            int lo = 0, hi = a.batch - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (s_end[mid] * per_b > u) hi = mid; else lo = mid + 1;
+            }
+            b = lo;
+            const int first = b > 0 ? s_end[b - 1] : 0;
+            const uint32_t before = first * per_b;
+            n = s_end[b] - first;
+            pr = (u - before) / n;
+            p0 = before + pr * n;
+            c0 = u - p0;
+            c1 = min(u_end, p0 + n) - p0;
         }
-        const int b = lo, first = b > 0 ? s_end[b - 1] : 0;
-        const uint32_t n = s_end[b] - first, before = first * per_b;
-        const uint32_t pr = (u - before) / n, p0 = before + pr * n;
         const int h = pr / a.row_blocks, rb = pr - h * a.row_blocks;
-        const int c0 = u - p0, c1 = min(u_end, p0 + n) - p0;
         const int pos = (int)a.position[a.per_sequence ? b : 0];
         const int len = pos + a.tokens;
 
@@ -783,7 +822,11 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 A.z = fmaf(x.z, f, A.z);
                 A.w = fmaf(x.w, f, A.w);
             }
-            if (whole) {
+            if (CL) {  // over warp 0's sums and statistics of this row, which are used up
+                __syncwarp();
+                *reinterpret_cast<float4*>(s_o + r * kQ8OPitch + 4 * lane) = A;
+                if (lane == 0) *reinterpret_cast<float4*>(s_stat[0][r]) = make_float4(M, Y, L, 0.f);
+            } else if (whole) {
                 const int rr = rb * a.rows + r, tok = rr * a.g_mul >> 16, hh = rr - tok * a.G;
                 const float f = (Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift)) / L;
                 *reinterpret_cast<uint2*>(
@@ -795,9 +838,48 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 if (lane == 0) *reinterpret_cast<float4*>(p + kHeadDim) = make_float4(M, Y, L, 0.f);
             }
         }
+        if (CL) {  // rows shared out among the cluster's warps, the CTAs' parts in order of their slots
+            cluster_arrive();
+            cluster_wait();
+            const int C = 1 << a.lg_cluster;
+            for (int r = (blockIdx.x & (C - 1)) * 4 + warp; r < rows; r += 4 * C) {
+                const uint32_t oa = smem0 + (r * kQ8OPitch + 4 * lane) * 4;
+                const uint32_t sa = static_cast<uint32_t>(__cvta_generic_to_shared(s_stat[0][r]));
+                float4 x[kQ8MaxCluster], st[kQ8MaxCluster];
+#pragma unroll
+                for (int k = 0; k < kQ8MaxCluster; ++k) {
+                    st[k] = k < C ? ld_cluster_f4(sa, k) : make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+                    x[k] = k < C ? ld_cluster_f4(oa, k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                float M = -INFINITY, Y = -INFINITY, L = 0.f;
+                float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < kQ8MaxCluster; ++k) {
+                    M = fmaxf(M, st[k].x);
+                    Y = fmaxf(Y, st[k].y);
+                }
+#pragma unroll
+                for (int k = 0; k < kQ8MaxCluster; ++k) {
+                    L += st[k].z * q8_weight(st[k].x, M);
+                    const float f = q8_weight(st[k].y, Y);
+                    A.x = fmaf(x[k].x, f, A.x);
+                    A.y = fmaf(x[k].y, f, A.y);
+                    A.z = fmaf(x[k].z, f, A.z);
+                    A.w = fmaf(x[k].w, f, A.w);
+                }
+                const int rr = rb * a.rows + r, tok = rr * a.g_mul >> 16, hh = rr - tok * a.G;
+                const float f = (Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift)) / L;
+                *reinterpret_cast<uint2*>(
+                    a.out + (((int64_t)b * a.tokens + tok) * a.hq + (int64_t)h * a.G + hh) * kHeadDim +
+                    4 * lane) = make_uint2(bf16_pair(A.x * f, A.y * f), bf16_pair(A.z * f, A.w * f));
+            }
+            cluster_arrive();  // no CTA leaves while another may still read its shared memory
+            cluster_wait();
+            return;
+        }
         __syncthreads();  // the ring and the statistics may be written again
         u = p0 + c1;
-    }
+    } while (u < u_end);
 }
 
 // 2^lg_wpr warps per query row: adds the parts of a pair that several CTAs share (each warp its
@@ -910,6 +992,39 @@ static bool q8_block_ok(int block) {
 // sequences of 3000 slots, 32 rows), 185 against 177 (16 of 8192, 64 rows).
 static int q8_rows(int rows) { return rows <= 8 ? 8 : 16; }
 
+// The short-cache form: one launch of a cluster per pair.
+template <int NT>
+static int q8_launch_cluster(const Q8AttnArgs& a, cudaStream_t s) {
+    auto kernel = q8_attn_kernel<NT, true>;
+    static bool ready[64] = {};  // per device: the kernel's shared-memory limit is raised
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return NK_ERR_CUDA;
+    if (dev < 0 || dev >= 64) return NK_ERR_DEVICE;
+    if (!ready[dev]) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 q8_attn_smem(NT)) != cudaSuccess ||
+            cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 (int)cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+            return NK_ERR_CUDA;
+        ready[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((a.batch * a.hkv * a.row_blocks) << a.lg_cluster);
+    cfg.blockDim = dim3(kQ8AttnThreads);
+    cfg.dynamicSmemBytes = q8_attn_smem(NT);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1 << a.lg_cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? NK_OK : NK_ERR_CUDA;
+}
+
 template <int NT>
 static int q8_launch_attn(Q8AttnArgs a, cudaStream_t s) {
     static int slots[64] = {};  // CTAs resident at once, per device
@@ -918,12 +1033,12 @@ static int q8_launch_attn(Q8AttnArgs a, cudaStream_t s) {
     if (dev < 0 || dev >= 64) return NK_ERR_DEVICE;
     if (slots[dev] == 0) {
         int sms = 0, per_sm = 0;
-        if (cudaFuncSetAttribute(q8_attn_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        if (cudaFuncSetAttribute(q8_attn_kernel<NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  q8_attn_smem(NT)) != cudaSuccess ||
-            cudaFuncSetAttribute(q8_attn_kernel<NT>, cudaFuncAttributePreferredSharedMemoryCarveout,
+            cudaFuncSetAttribute(q8_attn_kernel<NT, false>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                  (int)cudaSharedmemCarveoutMaxShared) != cudaSuccess ||
             cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, q8_attn_kernel<NT>,
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, q8_attn_kernel<NT, false>,
                                                           kQ8AttnThreads, q8_attn_smem(NT)) !=
                 cudaSuccess ||
             per_sm < 1)
@@ -933,7 +1048,7 @@ static int q8_launch_attn(Q8AttnArgs a, cudaStream_t s) {
     const int64_t pairs = (int64_t)a.batch * a.hkv * a.row_blocks;
     const int64_t most = (int64_t)((a.capacity + kQ8Unit - 1) / kQ8Unit) * pairs;
     a.grid = (int)min((int64_t)slots[dev], most);
-    const int rc = launch_pdl_smem(q8_attn_kernel<NT>, dim3(a.grid), dim3(kQ8AttnThreads),
+    const int rc = launch_pdl_smem(q8_attn_kernel<NT, false>, dim3(a.grid), dim3(kQ8AttnThreads),
                                    (size_t)q8_attn_smem(NT), s, a);
     if (rc != NK_OK) return rc;
     // about grid / pairs parts to a row: up to eight warps share them, at least two each
@@ -1060,8 +1175,16 @@ extern "C" int nk_attention_decode_q8(const void* q, const nk_q8_cache* c,
     a.cs = c->seq_stride;
     a.scale_log2 = scale * 1.4426950408889634f;
     cudaStream_t s = (cudaStream_t)stream;
-    switch (a.rows) {
-        case 8: return q8_launch_attn<1>(a, s);
-        default: return q8_launch_attn<2>(a, s);
-    }
+    // The short-cache form with the largest cluster that leaves every CTA resident (384 of them, in
+    // clusters, of the three an SM), if a CTA then has at most 512 slots to walk. Measured (us, one
+    // launch / two): 8 pairs 5.1 / 7.4 at 1024 slots, 8.8 / 9.9 at 4096, 13.5 / 11.8 at 8192; 64 pairs
+    // (clusters of 4) 7.8 / 11.1 at 1024, 12.0 / 14.1 at 2048, 18.7 / 19.4 at 4096; 128 pairs (of 2)
+    // 7.8 / 11.0 at 512, 11.6 / 14.0 at 1024, 18.4 / 19.5 at 2048, with 16 rows 27.2 / 26.3; past one
+    // wave, 64 pairs in clusters of 8, 15.2 / 14.1 at 2048.
+    const int64_t pairs = (int64_t)a.batch * a.hkv * a.row_blocks;
+    for (int lg = 3; lg > 0 && !a.lg_cluster; --lg)
+        if (pairs << lg <= 384) a.lg_cluster = lg;
+    const bool cluster = a.lg_cluster && a.capacity <= 512 << a.lg_cluster;
+    if (a.rows == 8) return cluster ? q8_launch_cluster<1>(a, s) : q8_launch_attn<1>(a, s);
+    return cluster ? q8_launch_cluster<2>(a, s) : q8_launch_attn<2>(a, s);
 }

@@ -135,6 +135,23 @@ def test_attention_ragged_batches(B, S):
     assert nk.device_error() == 0
 
 
+@pytest.mark.parametrize("B", (1, 5, 6, 7, 12, 13, 24, 25))
+@pytest.mark.parametrize("T,heads", [(1, 32), (3, 32), (4, 64)])
+def test_attention_short_and_long_capacities(B, T, heads):
+    """The same slots at the start of a short cache and of a long one: the launch depends on the
+    capacity and on how many (sequence, kv head) pairs there are."""
+    long = filled_cache(B, 8, 4608, 64, seed=B)
+    for S in (192, 1024):
+        short = ops.Q8Cache(long.k[:, :, :S], long.v[:, :, :S],
+                            long.k_scale[:, :, :S // 64].clone(), long.v_scale[:, :, :S // 64].clone(), 64)
+        pos = [(S - T) * (b + 1) // B for b in range(B)]
+        if B > 5:
+            pos[2], pos[4] = -1, 0
+        q = rand(B * T, heads * 128, seed=S + T)
+        for cache in (short, long):
+            check_attention(q, cache, pos, heads)
+
+
 def test_attention_shared_position_and_scale():
     cache = filled_cache(4, 8, 512, 32, seed=3)
     q = rand(4, 32 * 128, seed=4)
