@@ -414,8 +414,10 @@ q8_attn_kernel(const Q8AttnArgs a) {
     __shared__ float s_stat[4][8 * NT][4];
     __shared__ uint2 s_q[NT > 1 ? NT * 8 * 32 : 1];     // Q^T operand, shared by the warps
     __shared__ float s_down[8 * NT];                    // and its rows' powers of two
-    if (threadIdx.x == 0) griddep_launch_dependents();
+    // in this order: the joining launch reads the positions ahead of its wait for this one, and so
+    // must not start before what wrote them has finished
     griddep_wait();
+    if (threadIdx.x == 0) griddep_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const uint32_t per_b = a.hkv * a.row_blocks;        // pairs per sequence
@@ -887,7 +889,6 @@ q8_attn_kernel(const Q8AttnArgs a) {
 __global__ void __launch_bounds__(32 * kQ8MergeWarps) q8_merge_kernel(const Q8AttnArgs a) {
     __shared__ float4 s_a[kQ8MergeWarps][32], s_st[kQ8MergeWarps];
     if (threadIdx.x == 0) griddep_launch_dependents();
-    griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int wpr = 1 << a.lg_wpr, sub = warp & (wpr - 1);
     const int b = blockIdx.y;
@@ -910,14 +911,15 @@ __global__ void __launch_bounds__(32 * kQ8MergeWarps) q8_merge_kernel(const Q8At
     const uint32_t per_b = a.hkv * a.row_blocks;
     uint2* out = reinterpret_cast<uint2*>(
         a.out + (((int64_t)b * a.tokens + tok) * a.hq + head) * kHeadDim + 4 * lane);
-    if (n == 0) return;  // idle: the first launch wrote the zeros
     const uint32_t U = all * per_b;
-    const Q8Split split(U, min((uint32_t)a.grid, U));
+    const Q8Split split(U, max(min((uint32_t)a.grid, U), 1u));
     const uint32_t p0 = before * per_b + (h * a.row_blocks + rb) * n;
     const int cf = live ? split.cta_of(p0) : 0, cl = live ? split.cta_of(p0 + n - 1) : 0;
     const bool shared_pair = cf != cl;  // (else that CTA wrote the row, or there is no row)
     const int parts = cl - cf + 1;
     const int i0 = sub * parts >> a.lg_wpr, i1 = (sub + 1) * parts >> a.lg_wpr;
+    griddep_wait();  // all of the above is on hand when the first launch ends
+    if (n == 0) return;  // idle: the first launch wrote the zeros
     float M = -INFINITY, Y = -INFINITY, L = 0.f;
     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
     if (shared_pair) {
