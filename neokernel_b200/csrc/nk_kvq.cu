@@ -283,15 +283,17 @@ __global__ void __launch_bounds__(32 * kQ8Warps) q8_append_kernel(const Q8Append
 //
 // A pair covered by one CTA is written directly; otherwise its CTAs write (m, my, l, O) of their
 // part, and a second launch adds the parts in order of their slots, its rows spread over the
-// GPU. (Measured: the last CTA of a pair adding the parts in the first launch instead takes
+// GPU; it works out where its parts lie before it waits for the first (20.5 -> 18.8 us at five
+// sequences of 3000 with 32 query rows). (Measured: the last CTA of a pair adding the parts in the first launch instead takes
 // 11.2 us where the two launches took 8.5, at one sequence of 1024 slots, and 60 where they took
 // 30 at five of 3000 with 32 query rows: one CTA walks through all rows of the pair.)
 //
-// Measured, 8 kv heads (us, both launches; in brackets the cache's bytes at 6456 GB/s): two
-// sequences of 128k slots 86.4 [83.2], 6.2 TB/s; 16 ragged ones of up to 8192 slots 32.6 [22.0]; one
-// of 1024 slots (a cluster per pair) 5.0 [0.3]; five of up to 3000, four tokens x 64 heads, 20.4 [2.8]. Long caches
-// stream at the copy rate; the fixed part (first bytes, join; two launches) is some 4 to 7 us; many
-// query rows are bound by the conversions and the matrix instructions (issue slots 45% busy).
+// Measured, 8 kv heads (us, all launches; in brackets the cache's bytes at 6456 GB/s): two
+// sequences of 128k slots 85.5 [83.2], 6.3 TB/s; 16 ragged ones of up to 8192 slots 31.5 [22.0]; one
+// of 1024 slots (a cluster per pair) 5.0 [0.3]; five of up to 2999, four tokens x 64 heads, 18.8
+// [2.8]. Long caches stream at the copy rate; the fixed part (first bytes, join, two launches) is
+// some 4 to 6 us; many query rows are bound by the conversions and the matrix instructions (issue
+// slots 45% busy at 12 warps an SM).
 // ---------------------------------------------------------------------------------------
 constexpr int kQ8Unit = 64;                 // slots per unit, 16 per warp
 constexpr int kQ8AttnThreads = 128;
@@ -1178,11 +1180,11 @@ extern "C" int nk_attention_decode_q8(const void* q, const nk_q8_cache* c,
     a.scale_log2 = scale * 1.4426950408889634f;
     cudaStream_t s = (cudaStream_t)stream;
     // The short-cache form with the largest cluster that leaves every CTA resident (384 of them, in
-    // clusters, of the three an SM), if a CTA then has at most 512 slots to walk. Measured (us, one
-    // launch / two): 8 pairs 5.1 / 7.4 at 1024 slots, 8.8 / 9.9 at 4096, 13.5 / 11.8 at 8192; 64 pairs
-    // (clusters of 4) 7.8 / 11.1 at 1024, 12.0 / 14.1 at 2048, 18.7 / 19.4 at 4096; 128 pairs (of 2)
-    // 7.8 / 11.0 at 512, 11.6 / 14.0 at 1024, 18.4 / 19.5 at 2048, with 16 rows 27.2 / 26.3; past one
-    // wave, 64 pairs in clusters of 8, 15.2 / 14.1 at 2048.
+    // clusters, at three CTAs an SM), if a CTA then has at most 512 slots to walk. Measured (us, one
+    // launch / two): 8 pairs 5.0 / 6.0 at 1024 slots, 8.6 / 8.9 at 4096, 10.7 / 10.7 at 6000; 64 pairs
+    // (clusters of 4) 7.9 / 10.0 at 1024, 12.1 / 12.9 at 2048, 18.8 / 18.2 at 4096; 128 pairs (of 2)
+    // 7.7 / 9.8 at 512, 11.9 / 12.8 at 1024, 18.7 / 18.3 at 2048; past one wave, 64 pairs in
+    // clusters of 8, 15.2 / 12.9 at 2048.
     const int64_t pairs = (int64_t)a.batch * a.hkv * a.row_blocks;
     for (int lg = 3; lg > 0 && !a.lg_cluster; --lg)
         if (pairs << lg <= 384) a.lg_cluster = lg;
