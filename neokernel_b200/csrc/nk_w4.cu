@@ -138,6 +138,18 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint
         : "memory");
 }
 
+// 32 lanes x 8 consecutive columns of tensor memory -> 8 registers per thread, there after
+// tcgen05.wait::ld; loaded() keeps uses of them behind that wait.
+__device__ __forceinline__ void tmem_ld8_async(uint32_t taddr, float (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]),
+                   "=f"(v[6]), "=f"(v[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void loaded(float (&v)[8]) {
+    asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]),
+                      "+f"(v[6]), "+f"(v[7])::"memory");
+}
+
 // 16 registers per thread -> 32 lanes x 16 consecutive 32-bit columns of tensor memory.
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
@@ -326,7 +338,8 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
                                   bdesc + (((kk >> 2) * (NT * 128) + 32 * (kk & 3)) >> 4), idesc,
                                   k > 0);
                     }
-                    tc_commit(j == NG - 1 ? bar_done + 8 * xs : bar_group + 8 * (kByAcc ? db : j));
+                    if (j == NG - 1) tc_commit(bar_done + 8 * xs);
+                    else if (!L::kStepRelease) tc_commit(bar_group + 8 * (kByAcc ? db : j));
                 }
                 __syncwarp();
                 if (++db == DB) {
@@ -432,29 +445,53 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
                 st = 0;
                 wph ^= 1;
             }
-#pragma unroll
-            for (int j = 0; j < NG; ++j) {
-                ok = __all_sync(0xffffffffu,
-                                j == NG - 1 ? w4_wait(bar_done + 8 * xs, xph)
-                                            : w4_wait(bar_group + 8 * (kByAcc ? db : j),
-                                                      kByAcc ? dph : i & 1));
+            if constexpr (L::kStepRelease) {
+                // the step's groups together: one wait and one round trip to tensor memory per eight
+                // tokens, none for columns past the last token
+                ok = __all_sync(0xffffffffu, w4_wait(bar_done + 8 * xs, xph));
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < COLS; c += 16) {
-                    float v[16];
-                    tmem_ld16(taddr + db * NT + c, v);
+                for (int c = 0; c < COLS; c += 8) {
+                    if (half * COLS + c >= mcount) break;
+                    float v[NG][8];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(s[j], v[e], acc[c + e]);
+                    for (int j = 0; j < NG; ++j) tmem_ld8_async(taddr + (db + j) * NT + c, v[j]);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int j = 0; j < NG; ++j) {
+                        loaded(v[j]);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) acc[c + e] = fmaf(s[j], v[j][e], acc[c + e]);
+                    }
                 }
                 tc_fence_before();
-                if (!L::kStepRelease) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar_free + 8 * db);
-                }
-                if (++db == DB) {
-                    db = 0;
-                    dph ^= 1;
+                if ((db += NG) == DB) db = 0;
+            } else {
+#pragma unroll
+                for (int j = 0; j < NG; ++j) {
+                    ok = __all_sync(0xffffffffu,
+                                    j == NG - 1 ? w4_wait(bar_done + 8 * xs, xph)
+                                                : w4_wait(bar_group + 8 * (kByAcc ? db : j),
+                                                          kByAcc ? dph : i & 1));
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < COLS; c += 16) {
+                        float v[16];
+                        tmem_ld16(taddr + db * NT + c, v);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(s[j], v[e], acc[c + e]);
+                    }
+                    tc_fence_before();
+                    if (!L::kStepRelease) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar_free + 8 * db);
+                    }
+                    if (++db == DB) {
+                        db = 0;
+                        dph ^= 1;
+                    }
                 }
             }
             if (L::kStepRelease) {
