@@ -15,9 +15,9 @@
 // MMA's A operand there (128 rows = 128 lanes), the tokens its B operand in shared memory.
 //
 // Measured in CUDA graphs (us; in brackets the weight bytes' time at 6456 GB/s, the copy rate):
-//   N 24576, K 4096   M=1 16.1 [8.0], M=64 26.4 [8.3]     group 128
-//   N 6144, K 4096    M=16 8.0 [2.1]                      group 64
-//   N 4096, K 12288   M=8 12.9 [4.7]                      group 32 with zero points
+//   N 24576, K 4096   M=1 16.1 [8.0], M=64 24.8 [8.3]     group 128
+//   N 6144, K 4096    M=16 7.8 [2.1]                      group 64
+//   N 4096, K 12288   M=8 11.6 [4.7]                      group 32 with zero points
 //   N 1024, K 2048    M=1 3.4 [0.2]: the launch and one pass through the pipeline
 // Per step of 128 x 128 the eight MMAs take some 256 cycles (each reads 4 KB of A from tensor
 // memory at 128 bytes a cycle), and a step of a CTA 450 to 500, with its barriers. So what bounds
@@ -76,8 +76,9 @@ struct W4Smem {
     static constexpr int kAccs = NT == 16 ? 8 : (NT == 32 ? 4 : 2);  // accumulators in tensor memory
     static constexpr int kTmemA = 2 * 64;                     // two A buffers of 64 columns
     static constexpr int kTmemCols = 256;
-    // Where the accumulators hold two steps' groups, the fold warps' release of a step is one of
-    // the arrivals that a later step's MMAs wait for; else the MMAs wait for each accumulator.
+    // Where the accumulators hold two steps' groups, the fold warps take a step's groups together,
+    // and their release of it is one of the arrivals that a later step's MMAs wait for; else they
+    // take each group as it is summed, and the MMAs wait for each accumulator.
     static constexpr bool kStepRelease = kAccs >= 2 * NG;
     static constexpr int kLag = kAccs / NG;                   // steps from a release to its reuse
     static constexpr int kGroupBars = kAccs > 4 ? kAccs : 4;  // group barriers (see the kernel)
@@ -476,18 +477,31 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
                                                           kByAcc ? dph : i & 1));
                     if (!ok) break;
                     tc_fence_after();
+                    // (eight tokens a trip for the 64-token tile, whose registers are full, 16 for 32:
+                    // measured 45.5 against 46.7 us, and 33.1 against 29.4; N 24576, K 4096, group 32)
+                    if constexpr (FH == 2) {
 #pragma unroll
-                    for (int c = 0; c < COLS; c += 16) {
-                        float v[16];
-                        tmem_ld16(taddr + db * NT + c, v);
+                        for (int c = 0; c < COLS; c += 8) {
+                            if (half * COLS + c >= mcount) break;
+                            float v[8];
+                            tmem_ld8_async(taddr + db * NT + c, v);
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                            loaded(v);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(s[j], v[e], acc[c + e]);
+                            for (int e = 0; e < 8; ++e) acc[c + e] = fmaf(s[j], v[e], acc[c + e]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < COLS; c += 16) {
+                            float v[16];
+                            tmem_ld16(taddr + db * NT + c, v);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(s[j], v[e], acc[c + e]);
+                        }
                     }
                     tc_fence_before();
-                    if (!L::kStepRelease) {
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(bar_free + 8 * db);
-                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_free + 8 * db);
                     if (++db == DB) {
                         db = 0;
                         dph ^= 1;
@@ -727,7 +741,7 @@ extern "C" int nk_gemm_w4(const void* x, int64_t ldx, const nk_w4_weight* w, voi
     const bool fp16 = w->scale_type == NK_W4_SCALE_FP16;
     cudaStream_t s = (cudaStream_t)stream;
     // the narrowest token tile that holds M (a wider one costs MMA columns, fold registers and ring
-    // stages: N 24576, K 4096 takes 16.1 us with 16 columns, 26.4 with 64); beyond 64 tokens the
+    // stages: N 24576, K 4096 takes 16.1 us with 16 columns, 18.8 with 32, 24.8 with 64); beyond 64 tokens the
     // weights are read once per 64
     if (M <= 16) return w4_dispatch<16>(a, group, fp16, s);
     if (M <= 32) return w4_dispatch<32>(a, group, fp16, s);
