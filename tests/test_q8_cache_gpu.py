@@ -496,3 +496,23 @@ def test_cache_refuses_shared_arrays():
         ops.Q8Cache(c.k, c.v, c.k_scale, c.k_scale, 64)
     both = torch.zeros(1, 2, 64, 2, 128, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
     ops.Q8Cache(both[..., 0, :], both[..., 1, :], c.k_scale, c.v_scale, 64)  # side by side
+
+
+@pytest.mark.parametrize("S", (1024, 6000))  # a cluster per pair; the partition and its join
+def test_attention_on_two_streams_at_once(S):
+    caches = [filled_cache(3, 8, S, 64, seed=n) for n in (1, 2)]
+    qs = [rand(3, 32 * 128, seed=n) for n in (3, 4)]
+    pos = torch.tensor([S - 1, -1, S // 3], device=DEV)
+    want = [run_attention(q, c, pos.tolist(), 32) for q, c in zip(qs, caches)]
+    outs = [[torch.full_like(q, float("nan")) for _ in range(20)] for q in qs]
+    ws = [ops.attention_q8_workspace(c, 32) for c in caches]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for n, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                ops.attention_decode_q8(qs[n], caches[n], pos, outs[n][i], ws[n], 32)
+    torch.cuda.synchronize()
+    for n in range(2):
+        for out in outs[n]:
+            assert torch.equal(out.view(torch.int16), want[n].view(torch.int16))
