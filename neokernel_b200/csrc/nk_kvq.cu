@@ -273,15 +273,19 @@ __global__ void __launch_bounds__(32 * kQ8Warps) q8_append_kernel(const Q8Append
 // running maxima. O^T += V^T P^T: V^T comes from transposed 8x8 loads of byte pairs, P^T from
 // transposing the probabilities' registers (movmatrix).
 //
-// The value scale differs between blocks, so it cannot be taken out of the sum: probabilities
-// are 2^(x + log2 s_v - my) with a running maximum my of x + log2 s_v of their own, rounded
-// to f16 (11 bits, from 2^15 down to 2^-24: what underflows is below 2^-39 of the largest
-// term), while the sum l = sum 2^(x - m) stays in fp32. Then out = (O / l) 2^(my - m).
+// The value scale differs between blocks, so it cannot be taken out of the sum. A warp holds O in a
+// unit 2^U next to the scales it meets: the matrix instruction takes p = 2^(x - m) times
+// c = 2^14 s_v / 2^U, and where a block's scale leaves [2^(U-6), 2^(U+1)) the unit moves to it and O is
+// multiplied by the power of two between them. So what a probability loses in f16 goes by the
+// probability alone, whatever scales (of blocks whose codes may all be 0) stand beside its own: 11
+// bits down to 2^-22 of the row's largest (2^-14 in f16, c at least 2^8), absolutely 2^-33 of the
+// largest below that. The unit stays within 2^64 of the largest scale seen (O must not overflow in
+// fp32: 2^15 2^9 a term and up to 2^30 terms). l = sum 2^(x - m) stays in fp32, and out = (O / l) 2^(U - 14).
 //
 // Short caches take the same walk in another frame: a cluster of CTAs per pair, joined through
 // distributed shared memory in one launch (the rule and its figures are in nk_attention_decode_q8).
 //
-// A pair covered by one CTA is written directly; otherwise its CTAs write (m, my, l, O) of their
+// A pair covered by one CTA is written directly; otherwise its CTAs write (m, U, l, O) of their
 // part, and a second launch adds the parts in order of their slots, its rows spread over the
 // GPU; it works out where its parts lie before it waits for the first (20.5 -> 18.8 us at five
 // sequences of 3000 with 32 query rows). (Measured: the last CTA of a pair adding the parts in the first launch instead takes
@@ -309,8 +313,11 @@ __host__ __device__ constexpr int q8_scale_off(int nt) {
 }
 __host__ __device__ constexpr int q8_attn_smem(int nt) { return q8_scale_off(nt) + 4 * kQ8Stages * 8; }
 constexpr int kQ8MaxGrid = 148 * 4;
-constexpr int kQ8PartFloats = kHeadDim + 4; // O, then m, my, l
-constexpr float kQ8Shift = 15.f;            // probabilities are held times 2^15
+constexpr int kQ8PartFloats = kHeadDim + 4; // O, then m, U, l
+constexpr int kQ8Shift = 14;                // c of a scale in the unit's own binade is in [2^14, 2^15)
+constexpr int kQ8UnitBelow = 6;             // binades below the unit that a scale may lie in
+constexpr int kQ8UnitRange = 64;            // and the unit below the largest scale seen
+constexpr int kQ8LeastUnit = -100;          // also where a warp begins; the append's scales are 2^-64 or more
 constexpr int kQ8MergeWarps = 8;
 constexpr int kQ8MaxCluster = 8;
 
@@ -370,18 +377,16 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// 2^x and log2 x by the special-function unit (2^x: relative error 2^-22; results below 2^-126 are
-// 0; log2 of a power of two is off by 2^-22 of it at most: both far below the 2^-11 of the f16
-// probabilities).
+// 2^x by the special-function unit (relative error 2^-22, far below the 2^-11 of the f16
+// probabilities; results below 2^-126 are 0).
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float lg2(float x) {
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+// 2^k, 0 for k < -126.
+__device__ __forceinline__ float q8_pow2(int k) {
+    return __uint_as_float((uint32_t)(max(k, -127) + 127) << 23);
 }
 // Factor of a part with running maximum m where all parts have maximum M. A part that saw nothing
 // (m = -inf) has sums of 0, or NaN if what it saw was NaN: 1 keeps both.
@@ -607,14 +612,13 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 last[nt][i] = rr < total_rows ? rr * a.g_mul >> 16 : -1;
             }
 
-        // m, my: running maxima of x and x + log2 s_v; ref, off: what the exponents subtract (0 while
-        // nothing was seen)
-        float m[NT][2], my[NT][2], ref[NT][2], off[NT][2], l[NT][2], o[8][NT][4];
+        // m: running maximum of x; ref: what the exponents subtract (0 while nothing was seen)
+        float m[NT][2], ref[NT][2], l[NT][2], o[8][NT][4];
+        int unit = kQ8LeastUnit, unit_max = kQ8LeastUnit;  // U, and the largest scale's exponent so far
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            m[nt][0] = m[nt][1] = my[nt][0] = my[nt][1] = -INFINITY;
+            m[nt][0] = m[nt][1] = -INFINITY;
             ref[nt][0] = ref[nt][1] = l[nt][0] = l[nt][1] = 0.f;
-            off[nt][0] = off[nt][1] = kQ8Shift;
 #pragma unroll
             for (int d = 0; d < 8; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
         }
@@ -633,7 +637,14 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 float k_scale, v_scale;
                 asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(k_scale), "=f"(v_scale)
                              : "r"(s_scale + stage * 8) : "memory");
-                const float v_log2 = lg2(v_scale);
+                // the unit that this block asks for (one of scale 0 leaves it), ahead of the scores
+                const int ve = max((int)(__float_as_uint(v_scale) >> 23 & 0xff) - 127, kQ8LeastUnit);
+                const bool moves = v_scale != 0.f && (uint32_t)(unit - ve) > (uint32_t)kQ8UnitBelow;
+                if (moves) unit_max = max(unit_max, ve);
+                const int next_unit = moves ? max(ve, unit_max - kQ8UnitRange) : unit;
+                const float moved = q8_pow2(unit - next_unit);
+                const float up = v_scale * q8_pow2(kQ8Shift - next_unit);  // c
+                unit = next_unit;
                 float s[NT][4];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
@@ -656,7 +667,7 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 }
                 // scores of slots j0 + g and j0 + 8 + g against rows 2t, 2t + 1
                 const bool all_seen = j0 + 15 <= pos;
-                bool grown = false;
+                bool grown = moves;
                 float mx[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -674,24 +685,21 @@ q8_attn_kernel(const Q8AttnArgs a) {
                         y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
                         y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
                         mx[nt][e] = y;
-                        grown |= y > m[nt][e] || y + v_log2 > my[nt][e];
+                        grown |= y > m[nt][e];
                     }
                 }
-                if (__any_sync(0xffffffffu, grown)) {  // a new maximum: rescale the sums
+                if (__any_sync(0xffffffffu, grown)) {  // a new maximum or unit: rescale the sums
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float al[2];
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const float mn = fmaxf(m[nt][e], mx[nt][e]);
-                            const float yn = fmaxf(my[nt][e], mx[nt][e] + v_log2);
                             ref[nt][e] = mn == -INFINITY ? 0.f : mn;
-                            const float yref = yn == -INFINITY ? 0.f : yn;
-                            l[nt][e] *= ex2(m[nt][e] - ref[nt][e]);
-                            al[e] = ex2(my[nt][e] - yref);
-                            off[nt][e] = kQ8Shift - yref;
+                            const float w = ex2(m[nt][e] - ref[nt][e]);
+                            l[nt][e] *= w;
+                            al[e] = w * moved;
                             m[nt][e] = mn;
-                            my[nt][e] = yn;
                         }
 #pragma unroll
                         for (int d = 0; d < 8; ++d) {
@@ -708,11 +716,10 @@ q8_attn_kernel(const Q8AttnArgs a) {
                     float f[2][2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float x0 = s[nt][e], x1 = s[nt][e + 2];
-                        const float up = v_log2 + off[nt][e];
-                        l[nt][e] += ex2(x0 - ref[nt][e]) + ex2(x1 - ref[nt][e]);
-                        f[0][e] = ex2(x0 + up);
-                        f[1][e] = ex2(x1 + up);
+                        const float p0 = ex2(s[nt][e] - ref[nt][e]), p1 = ex2(s[nt][e + 2] - ref[nt][e]);
+                        l[nt][e] += p0 + p1;
+                        f[0][e] = p0 * up;
+                        f[1][e] = p1 * up;
                     }
                     pf[nt][0] = movm_t(pack_f16x2(f[0][0], f[0][1]));
                     pf[nt][1] = movm_t(pack_f16x2(f[1][0], f[1][1]));
@@ -785,7 +792,7 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 x += __shfl_xor_sync(0xffffffffu, x, 16);
                 if (g == 0)
                     *reinterpret_cast<float4*>(s_stat[warp][8 * nt + 2 * t + i]) =
-                        make_float4(m[nt][i], my[nt][i], x, 0.f);
+                        make_float4(m[nt][i], (float)unit, x, 0.f);
             }
         __syncthreads();  // statistics are there; every warp is done with its ring
         float* s_o = reinterpret_cast<float*>(q8_smem);  // [warp][row][128]
@@ -806,7 +813,7 @@ q8_attn_kernel(const Q8AttnArgs a) {
         const int rows = min(8 * NT, total_rows - rb * a.rows);
         for (int r = warp; r < rows; r += 4) {
             float4 st[4];
-            float M = -INFINITY, Y = -INFINITY;
+            float M = -INFINITY, Y = kQ8LeastUnit;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 st[w] = *reinterpret_cast<const float4*>(s_stat[w][r]);
@@ -817,8 +824,8 @@ q8_attn_kernel(const Q8AttnArgs a) {
             float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                L += st[w].z * q8_weight(st[w].x, M);
-                const float f = q8_weight(st[w].y, Y);
+                const float p = q8_weight(st[w].x, M), f = p * ex2(st[w].y - Y);
+                L += st[w].z * p;
                 const float4 x = *reinterpret_cast<const float4*>(
                     s_o + (w * 8 * NT + r) * kQ8OPitch + 4 * lane);
                 A.x = fmaf(x.x, f, A.x);
@@ -832,7 +839,7 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 if (lane == 0) *reinterpret_cast<float4*>(s_stat[0][r]) = make_float4(M, Y, L, 0.f);
             } else if (whole) {
                 const int rr = rb * a.rows + r, tok = rr * a.g_mul >> 16, hh = rr - tok * a.G;
-                const float f = (Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift)) / L;
+                const float f = ex2(Y - kQ8Shift) / L;
                 *reinterpret_cast<uint2*>(
                     a.out + (((int64_t)b * a.tokens + tok) * a.hq + (int64_t)h * a.G + hh) * kHeadDim +
                     4 * lane) = make_uint2(bf16_pair(A.x * f, A.y * f), bf16_pair(A.z * f, A.w * f));
@@ -852,10 +859,10 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 float4 x[kQ8MaxCluster], st[kQ8MaxCluster];
 #pragma unroll
                 for (int k = 0; k < kQ8MaxCluster; ++k) {
-                    st[k] = k < C ? ld_cluster_f4(sa, k) : make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+                    st[k] = k < C ? ld_cluster_f4(sa, k) : make_float4(-INFINITY, kQ8LeastUnit, 0.f, 0.f);
                     x[k] = k < C ? ld_cluster_f4(oa, k) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
-                float M = -INFINITY, Y = -INFINITY, L = 0.f;
+                float M = -INFINITY, Y = kQ8LeastUnit, L = 0.f;
                 float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int k = 0; k < kQ8MaxCluster; ++k) {
@@ -864,15 +871,15 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 }
 #pragma unroll
                 for (int k = 0; k < kQ8MaxCluster; ++k) {
-                    L += st[k].z * q8_weight(st[k].x, M);
-                    const float f = q8_weight(st[k].y, Y);
+                    const float p = q8_weight(st[k].x, M), f = p * ex2(st[k].y - Y);
+                    L += st[k].z * p;
                     A.x = fmaf(x[k].x, f, A.x);
                     A.y = fmaf(x[k].y, f, A.y);
                     A.z = fmaf(x[k].z, f, A.z);
                     A.w = fmaf(x[k].w, f, A.w);
                 }
                 const int rr = rb * a.rows + r, tok = rr * a.g_mul >> 16, hh = rr - tok * a.G;
-                const float f = (Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift)) / L;
+                const float f = ex2(Y - kQ8Shift) / L;
                 *reinterpret_cast<uint2*>(
                     a.out + (((int64_t)b * a.tokens + tok) * a.hq + (int64_t)h * a.G + hh) * kHeadDim +
                     4 * lane) = make_uint2(bf16_pair(A.x * f, A.y * f), bf16_pair(A.z * f, A.w * f));
@@ -922,7 +929,7 @@ __global__ void __launch_bounds__(32 * kQ8MergeWarps) q8_merge_kernel(const Q8At
     const int i0 = sub * parts >> a.lg_wpr, i1 = (sub + 1) * parts >> a.lg_wpr;
     griddep_wait();  // all of the above is on hand when the first launch ends
     if (n == 0) return;  // idle: the first launch wrote the zeros
-    float M = -INFINITY, Y = -INFINITY, L = 0.f;
+    float M = -INFINITY, Y = kQ8LeastUnit, L = 0.f;
     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
     if (shared_pair) {
         for (int i = i0; i < i1; i += 4) {  // four parts' loads together
@@ -941,16 +948,16 @@ __global__ void __launch_bounds__(32 * kQ8MergeWarps) q8_merge_kernel(const Q8At
                 Mn = fmaxf(Mn, st[k].x);
                 Yn = fmaxf(Yn, st[k].y);
             }
-            L *= q8_weight(M, Mn);
-            const float fa = q8_weight(Y, Yn);
+            const float la = q8_weight(M, Mn), fa = la * ex2(Y - Yn);
+            L *= la;
             A.x *= fa; A.y *= fa; A.z *= fa; A.w *= fa;
             M = Mn;
             Y = Yn;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 if (i + k >= i1) break;
-                L += st[k].z * q8_weight(st[k].x, M);
-                const float f = q8_weight(st[k].y, Y);
+                const float p = q8_weight(st[k].x, M), f = p * ex2(st[k].y - Y);
+                L += st[k].z * p;
                 A.x = fmaf(x[k].x, f, A.x);
                 A.y = fmaf(x[k].y, f, A.y);
                 A.z = fmaf(x[k].z, f, A.z);
@@ -971,8 +978,8 @@ __global__ void __launch_bounds__(32 * kQ8MergeWarps) q8_merge_kernel(const Q8At
         A = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int w = 0; w < wpr; ++w) {
             const float4 st = s_st[warp + w], x = s_a[warp + w][lane];
-            L += st.z * q8_weight(st.x, M);
-            const float f = q8_weight(st.y, Y);
+            const float p = q8_weight(st.x, M), f = p * ex2(st.y - Y);
+            L += st.z * p;
             A.x = fmaf(x.x, f, A.x);
             A.y = fmaf(x.y, f, A.y);
             A.z = fmaf(x.z, f, A.z);
@@ -980,7 +987,7 @@ __global__ void __launch_bounds__(32 * kQ8MergeWarps) q8_merge_kernel(const Q8At
         }
     }
     if (!shared_pair) return;
-    const float f = (Y == -INFINITY ? 0.f : ex2(Y - M - kQ8Shift)) / L;
+    const float f = ex2(Y - kQ8Shift) / L;
     *out = make_uint2(bf16_pair(A.x * f, A.y * f), bf16_pair(A.z * f, A.w * f));
 }
 

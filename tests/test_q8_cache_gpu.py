@@ -516,3 +516,29 @@ def test_attention_on_two_streams_at_once(S):
     for n in range(2):
         for out in outs[n]:
             assert torch.equal(out.view(torch.int16), want[n].view(torch.int16))
+
+
+@pytest.mark.parametrize("S", (200, 1024, 6000))  # a cluster per pair; the partition and its join
+@pytest.mark.parametrize("T,heads", [(1, 4), (3, 16)])
+@pytest.mark.parametrize("power", (24, 45, 80))
+def test_attention_beside_a_large_scale_that_nothing_uses(S, T, heads, power):
+    """Blocks of zero codes whose value scale is 2^power times the others' (a large value that was
+    appended and overwritten leaves one behind) take nothing away from the rest.
+
+    Beside attention_ref's errors: what f16 loses of a probability below its normal range is
+    2^-33 of the row's largest, and the largest weighs 1 at most."""
+    H = 2
+    cache = filled_cache(2, H, S, 16, seed=S + power, lo=-8, hi=-4)
+    n = S // 16
+    for j in {0, 1, 2, 3, 5, n // 3, n // 2, n - 3, n - 1} | set(range(n // 2 + 8, n, 7)):
+        cache.v.view(torch.uint8)[:, :, 16 * j:16 * j + 16] = 0
+        cache.v_scale[:, :, j] = 2.0 ** (power - 6)
+    pos = [S - T, S // 2]
+    q = rand(2 * T, heads * 128, std=0.2, seed=power)
+    out = run_attention(q, cache, pos, heads)
+    ref, tol = attention_ref(q, cache, pos, heads)
+    v = cache.dequantize()[1].double().abs()
+    total = torch.stack([v[b, :, :p + T].sum(1) for b, p in enumerate(pos)])
+    tol = tol.view(2, T, heads, 128) + 2.0 ** -33 * total.repeat_interleave(heads // H, 1)[:, None]
+    off = (out.double() - ref).abs().view_as(tol)
+    assert (off <= tol).all(), (off / tol).max().item()
