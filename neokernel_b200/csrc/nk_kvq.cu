@@ -667,12 +667,14 @@ q8_attn_kernel(const Q8AttnArgs a) {
                 }
                 // scores of slots j0 + g and j0 + 8 + g against rows 2t, 2t + 1
                 const bool all_seen = j0 + 15 <= pos;
+                const bool big = k_scale > 0x1p64f;  // (s is below 2^30, qs 2^-103 or more)
                 bool grown = moves;
                 float mx[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[nt][e] = s[nt][e] * k_scale * qs[nt][e & 1];
+                    for (int e = 0; e < 4; ++e)  // neither order's first product passes fp32 unless the score does
+                        s[nt][e] = big ? s[nt][e] * qs[nt][e & 1] * k_scale : s[nt][e] * k_scale * qs[nt][e & 1];
                     if (!all_seen) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)

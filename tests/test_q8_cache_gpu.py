@@ -542,3 +542,30 @@ def test_attention_beside_a_large_scale_that_nothing_uses(S, T, heads, power):
     tol = tol.view(2, T, heads, 128) + 2.0 ** -33 * total.repeat_interleave(heads // H, 1)[:, None]
     off = (out.double() - ref).abs().view_as(tol)
     assert (off <= tol).all(), (off / tol).max().item()
+
+
+@pytest.mark.parametrize("power", (70, 100, 118))
+@pytest.mark.parametrize("tiny", (0, 80, 92))
+def test_attention_keys_next_to_the_largest(power, tiny):
+    """Keys of up to 2^126 against ordinary and tiny queries: scores of up to 2^55 past the others pick
+    out one slot, and no product on the way is larger than the score (nor lost where it is not).
+
+    Key codes are powers of two of one sign and each slot has one of its own, so that scores are
+    exact and no two are alike; queries are powers of two."""
+    S = 96
+    cache = filled_cache(1, 1, S, 32, seed=power)
+    k = torch.zeros(S, 128, device=DEV)
+    for j in range(S):
+        k[j, j] = 1.0 + (j % 8) / 8
+    cache.k.view(torch.uint8)[0, 0] = k.to(torch.float8_e4m3fn).view(torch.uint8)
+    cache.k_scale.fill_(2.0 ** power)
+    q = torch.zeros(2, 128, dtype=torch.bfloat16, device=DEV)
+    q[0] = 2.0 ** -tiny
+    q[1] = -2.0 ** -tiny
+    q[0, 71], q[1, 40] = 2.0 ** (1 - tiny), -2.0 ** (-1 - tiny)
+    out = run_attention(q.view(1, 256), cache, [S - 1], 2)
+    if power - tiny > 12:  # the runner-up is at least 2^(power - tiny) / 8 / sqrt(128) behind
+        want = cache.dequantize()[1][0, 0][[71, 40]]
+        assert torch.equal(out.view(2, 128).float(), want)
+    else:
+        check_attention(q.view(1, 256), cache, [S - 1], 2)
