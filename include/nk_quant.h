@@ -59,6 +59,12 @@ NK_API size_t nk_w4_zero_bytes(int N, int K, int group);
 NK_API int nk_gemm_w4(const void* x, int64_t ldx, const nk_w4_weight* w, void* y, int64_t ldy,
                       int M, nk_stream_t stream);
 
+/* Failure-detection tests only: CTA `cta` of the next nk_gemm_w4 launch (tiles of 128 rows first, a
+ * tile's CTAs side by side) never requests its last step's weights, so its waits for them expire (about 2 s).
+ * The tile's outputs are not written, whichever of its CTAs they fall to, the launch returns, and
+ * nk_device_error then reports NK_ERR_TIMEOUT. Consumed by that launch; -1 withholds nothing. */
+NK_API int nk_test_withhold_w4(int cta);
+
 /* ---- KV cache in 8 bits -------------------------------------------------------------------
  *
  * Keys and values are e4m3 codes (1 byte, finite range +-448) times a scale held for each

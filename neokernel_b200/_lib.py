@@ -43,6 +43,7 @@ EXPORTS = ("nk_plan_make", "nk_ws_bytes", "nk_ws_init", "nk_gemm_bf16", "nk_devi
            "nk_gemm_argmax_ws_bytes", "nk_gemm_bf16_argmax", "nk_test_withhold_partial",
            "nk_gemm_bf16_allreduce", "nk_gemm_bf16_qkv_rope_cache",
            "nk_w4_code_bytes", "nk_w4_scale_bytes", "nk_w4_zero_bytes", "nk_gemm_w4",
+           "nk_test_withhold_w4",
            "nk_qk_norm_rope_cache_q8", "nk_attention_q8_ws_bytes", "nk_attention_decode_q8")
 
 
@@ -188,6 +189,8 @@ def load() -> ctypes.CDLL:
     # the descriptors (nk_w4_weight, nk_q8_cache) go by address: one conversion a call
     L.nk_gemm_w4.argtypes = [vp, i64, vp, vp, i64, i32, vp]
     L.nk_gemm_w4.restype = i32
+    L.nk_test_withhold_w4.argtypes = [i32]
+    L.nk_test_withhold_w4.restype = i32
     L.nk_qk_norm_rope_cache_q8.argtypes = [vp, i64, vp, vp, vp, vp, vp, i32, vp, vp, i32, i32, f32,
                                            vp]
     L.nk_qk_norm_rope_cache_q8.restype = i32

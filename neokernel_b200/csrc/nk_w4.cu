@@ -42,7 +42,9 @@
 //
 // Every mbarrier wait is bounded: on expiry the thread records NK_ERR_TIMEOUT in the device error
 // word, its role ends, and the CTA drains its copies and MMAs (bounded), stores nothing, frees
-// its tensor memory and exits.
+// its tensor memory and exits. In a cluster no CTA stores anything of the tile then: its sum lacks a part.
+#include <atomic>
+
 #include "nk_common.cuh"
 #include "../../include/nk_quant.h"
 
@@ -62,7 +64,11 @@ struct W4Args {
     int M, N, K;
     int KB;                       // K steps of 128
     int wide_x;                   // x rows are 16-byte aligned: TMA reads them
+    int withhold;                 // failure-detection tests only (nk_test_withhold_w4), else -1
 };
+
+// CTA that the next launch's last step is withheld in; consumed by that launch.
+static std::atomic<int> g_withhold_w4{-1};
 
 template <int NT, int NG>
 struct W4Smem {
@@ -111,6 +117,11 @@ __device__ __forceinline__ void cluster_arrive() {
 }
 __device__ __forceinline__ void cluster_wait() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t saddr, uint32_t rank, uint32_t v) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t saddr, uint32_t rank) {
     uint32_t a;
@@ -235,6 +246,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
     const int mcount = min(NT, a.M - m0);
     const int k_begin = (int)((int64_t)rank * a.KB / S);
     const int n = (int)((int64_t)(rank + 1) * a.KB / S) - k_begin;  // steps, at least one
+    const int loads = n - (a.withhold == (int)(blockIdx.y * gridDim.x + blockIdx.x));
 
     const uint32_t bar_full = base + L::kBarOff;         // weights of a step have landed
     const uint32_t bar_empty = bar_full + WS * 8;        // ... and are used up
@@ -272,7 +284,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0)
-            for (int i = 0; i < min(n, WS); ++i) load_step(i, i);
+            for (int i = 0; i < min(loads, WS); ++i) load_step(i, i);
         __syncwarp();
     }
     if (warp == 1) {
@@ -300,7 +312,7 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
         if (lane == 0) {
             int st = 0, ph = 0;
 #pragma unroll 1
-            for (int i = WS; i < n; ++i) {
+            for (int i = WS; i < loads; ++i) {
                 if (!w4_wait(bar_empty + 8 * st, ph)) {
                     *abort_flag = 1u;
                     break;
@@ -602,10 +614,10 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
                      : "memory");
     }
     griddep_wait();  // outputs may still be read by the previous launch
-    const bool good = *abort_flag == 0u;
     const float* red = reinterpret_cast<const float*>(gbase);
     const int count = mcount * kW4Rows, n0 = tile * kW4Rows;
     if (S == 1) {
+        const bool good = *abort_flag == 0u;
         for (int e = threadIdx.x; e < count; e += kW4Threads) {
             const int m = e / kW4Rows, r = e % kW4Rows;
             if (good && n0 + r < a.N)
@@ -613,9 +625,12 @@ w4_kernel(const __grid_constant__ CUtensorMap tmap_x, const W4Args a) {
         }
         return;
     }
-    // each CTA of the cluster adds its share of the elements, in rank order
+    // each CTA of the cluster adds its share of the elements, in rank order; one whose waits expired
+    // has told the others
+    if (*abort_flag && threadIdx.x < S) st_cluster_u32(base + L::kMiscOff + 4, threadIdx.x, 1u);
     cluster_arrive();
     cluster_wait();
+    const bool good = *abort_flag == 0u;
     const int per = (count + S - 1) / S;
     for (int e = rank * per + threadIdx.x; e < min(count, (rank + 1) * per); e += kW4Threads) {
         float part[kW4MaxCluster];
@@ -738,6 +753,7 @@ extern "C" int nk_gemm_w4(const void* x, int64_t ldx, const nk_w4_weight* w, voi
     a.K = K;
     a.KB = (K + 127) / 128;
     a.wide_x = ((uintptr_t)x & 15u) == 0 && a.ldx % 8 == 0;
+    a.withhold = g_withhold_w4.exchange(-1);
     const bool fp16 = w->scale_type == NK_W4_SCALE_FP16;
     cudaStream_t s = (cudaStream_t)stream;
     // the narrowest token tile that holds M (a wider one costs MMA columns, fold registers and ring
@@ -746,4 +762,10 @@ extern "C" int nk_gemm_w4(const void* x, int64_t ldx, const nk_w4_weight* w, voi
     if (M <= 16) return w4_dispatch<16>(a, group, fp16, s);
     if (M <= 32) return w4_dispatch<32>(a, group, fp16, s);
     return w4_dispatch<64>(a, group, fp16, s);
+}
+
+extern "C" int nk_test_withhold_w4(int cta) {
+    if (cta < -1) return NK_ERR_ARG;
+    nk::g_withhold_w4.store(cta);
+    return NK_OK;
 }

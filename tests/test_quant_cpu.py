@@ -206,3 +206,9 @@ def test_quantize_refuses_what_has_no_scale():
     with pytest.raises(ValueError, match="finite"):
         nk.W4Weight.quantize(w, 32, scale_dtype=torch.float16)
     assert torch.isfinite(nk.W4Weight.quantize(w, 32).dequantize()).all()
+
+
+def test_withhold_w4_request_rejects_a_bad_cta():
+    L = _lib.load()
+    assert L.nk_test_withhold_w4(-2) == _lib.NK_ERR_ARG
+    assert L.nk_test_withhold_w4(-1) == 0

@@ -7,11 +7,13 @@ partials; taking every one of those additions (16 inside an instruction) as off 
 sum of magnitudes so far, |y - ref| <= eps_bf16 / 2 |ref| + (K + K / 32 + 64) 2^-23 sum |x w|.
 """
 
+import time
+
 import pytest
 import torch
 
 import neokernel_b200 as nk
-from neokernel_b200 import synthetic
+from neokernel_b200 import _lib, synthetic
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -162,3 +164,47 @@ def test_refusals():
         args = dict(a=x, w=W, out=y) | bad
         with pytest.raises(ValueError):
             nk.mm_w4(args["a"], args["w"], out=args["out"])
+
+
+# (M, N, K, group, CTAs of a tile): one CTA a tile; a cluster of eight, of three (two or three steps each) and
+# of two; each way in which the sums leave tensor memory
+@pytest.mark.parametrize("M,N,K,group,S", [(1, 24576, 512, 128, 1), (4, 4096, 4096, 64, 8),
+                                           (16, 4096, 896, 32, 3), (40, 12288, 1024, 32, 2)])
+def test_a_wait_that_runs_out_writes_nothing_of_its_tile(M, N, K, group, S):
+    """The CTA's waits expire (nothing faults or hangs), no CTA of its cluster stores sums that lack
+    its part, the error is reported, and the next call is right."""
+    L = _lib.load()
+    W, w = make(N, K, group, True, torch.bfloat16)
+    x = synthetic.activation(M, K, seed=M, device=DEV)
+    clean = torch.empty(M, N, dtype=torch.bfloat16, device=DEV)
+    nk.mm_w4(x, W, out=clean)
+    check(clean, x, w)
+    for tile, rank in ((1, 0), (2, S - 1)):
+        y = torch.full((M, N), 7.0, dtype=torch.bfloat16, device=DEV)
+        assert L.nk_test_withhold_w4(tile * S + rank) == 0
+        t0 = time.perf_counter()
+        nk.mm_w4(x, W, out=y)
+        torch.cuda.synchronize()
+        waited = time.perf_counter() - t0
+        assert nk.device_error() == _lib.NK_ERR_TIMEOUT
+        assert 1.0 <= waited <= 30.0, waited
+        rows = slice(128 * tile, 128 * tile + 128)
+        assert (y[:, rows] == 7.0).all(), "a tile without one of its parts was written"
+        y[:, rows] = clean[:, rows]
+        assert torch.equal(y, clean)
+        nk.mm_w4(x, W, out=y.fill_(7.0))  # the request was consumed
+        assert torch.equal(y, clean)
+        assert nk.device_error() == 0
+
+
+def test_withhold_request_is_validated():
+    L = _lib.load()
+    assert L.nk_test_withhold_w4(-2) == _lib.NK_ERR_ARG
+    assert L.nk_test_withhold_w4(5) == 0
+    assert L.nk_test_withhold_w4(-1) == 0  # cleared
+    W, w = make(256, 256, 128, False, torch.bfloat16)
+    x = synthetic.activation(2, 256, seed=1, device=DEV)
+    y = torch.empty(2, 256, dtype=torch.bfloat16, device=DEV)
+    nk.mm_w4(x, W, out=y)
+    check(y, x, w)
+    assert nk.device_error() == 0
