@@ -904,7 +904,6 @@ __global__ void __launch_bounds__(32 * kQ8MergeWarps) q8_merge_kernel(const Q8At
     const int wpr = 1 << a.lg_wpr, sub = warp & (wpr - 1);
     const int b = blockIdx.y;
     const int row = blockIdx.x * (kQ8MergeWarps >> a.lg_wpr) + (warp >> a.lg_wpr);  // t * hq + head
-    const bool live = row < a.tokens * a.hq;
     // units of the sequences before b, of b and of all
     uint32_t before = 0, all = 0;
 #pragma unroll 4
@@ -916,6 +915,7 @@ __global__ void __launch_bounds__(32 * kQ8MergeWarps) q8_merge_kernel(const Q8At
     before = __reduce_add_sync(0xffffffffu, before);
     all = __reduce_add_sync(0xffffffffu, all);
     const uint32_t n = q8_seq_units(a, b);
+    const bool live = n > 0 && row < a.tokens * a.hq;  // (an idle sequence has no units to look up)
     const int tok = row / a.hq, head = row - tok * a.hq;
     const int h = head / a.G, rr = tok * a.G + head - h * a.G;
     const int rb = rr / a.rows, r = rr - rb * a.rows;

@@ -569,3 +569,13 @@ def test_attention_keys_next_to_the_largest(power, tiny):
         assert torch.equal(out.view(2, 128).float(), want)
     else:
         check_attention(q.view(1, 256), cache, [S - 1], 2)
+
+
+@pytest.mark.parametrize("B", (1, 16, 65))
+def test_attention_all_idle_in_a_long_cache(B):
+    """No sequence has a unit of work, in the form of two launches."""
+    cache = filled_cache(B, 8, 8192 // (1 + B // 16), 64, seed=B)
+    poison(cache, [0] * B)
+    q = rand(2 * B, 16 * 128, seed=B)
+    assert (run_attention(q, cache, [-1 - b for b in range(B)], 16) == 0).all()
+    assert nk.device_error() == 0
