@@ -161,12 +161,28 @@ Q8_MAX_BATCH = 1024  # NK_Q8_MAX_BATCH
 Q8_BLOCKS = (16, 32, 64, 128)
 
 
+def _meets(dims, lo: int, hi: int) -> bool:
+    """Whether some sum of i * stride over the (stride, count) pairs ``dims`` (largest stride first),
+    0 <= i < count, lies strictly between ``lo`` and ``hi``."""
+    if not dims:
+        return lo < 0 < hi
+    (stride, count), rest = dims[0], dims[1:]
+    first = max(lo // stride + 1, 0)            # the least i whose own multiple is past lo
+    if first < count and first * stride < hi:
+        return True
+    reach = sum(s * (n - 1) for s, n in rest)   # smaller ones can still get there with the others' help
+    least = max((lo - reach) // stride + 1, 0)
+    return any(_meets(rest, lo - i * stride, hi - i * stride)
+               for i in range(least, min(first, count)))
+
+
 class Q8Cache:
     """A layer's KV cache in 8 bits: e4m3 codes ``k``, ``v`` [batch, kv_heads, capacity, 128] and
     fp32 scales ``k_scale``, ``v_scale`` [batch, kv_heads, ceil(capacity / block)]; the value held
     at slot j is ``k[..., j, :] * k_scale[..., j // block]``. The codes may have any batch, head
     and token strides that are multiples of 16, the same for ``k`` and ``v``; the scales are
-    contiguous. The tensors are the caller's and are read and written in place."""
+    contiguous, and no two of the four share memory (keys and values may lie between each other's rows,
+    as in one [.., 2, 128] tensor). The tensors are the caller's and are read and written in place."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "block", "batch", "kv_heads", "capacity",
                  "device", "_c", "_addr")
@@ -179,7 +195,6 @@ class Q8Cache:
                   "capacity, 128]")
         _need(v.shape == k.shape and v.stride() == k.stride() and v.device == k.device,
               "Q8Cache: k and v must have the same shape, strides and device")
-        _need(v.data_ptr() != k.data_ptr(), "Q8Cache: k and v must not share memory")
         _need(block in Q8_BLOCKS, f"Q8Cache: block must be one of {Q8_BLOCKS}, got {block}")
         B, H, S, _ = k.shape
         _need(1 <= B <= Q8_MAX_BATCH and H >= 1 and S >= 1,
@@ -198,8 +213,18 @@ class Q8Cache:
             _need(isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.device == k.device
                   and tuple(t.shape) == shape and t.is_contiguous(),
                   f"Q8Cache: scales must be contiguous fp32 {list(shape)} on the codes' device")
-        _need(k_scale.data_ptr() != v_scale.data_ptr(),
+        _need(abs(v_scale.data_ptr() - k_scale.data_ptr()) >= k_scale.nbytes,
               "Q8Cache: k_scale and v_scale must not share memory")
+        # rows of 128 bytes at these strides; between two of them, the differences of two indexes
+        dims = sorted(((st, n) for st, n in ((sb, B), (sh, H), (ss, S)) if n > 1), reverse=True)
+        mid = v.data_ptr() - k.data_ptr() + sum(st * (n - 1) for st, n in dims)
+        _need(not _meets([(st, 2 * n - 1) for st, n in dims], mid - HEAD_DIM, mid + HEAD_DIM),
+              "Q8Cache: k and v must not share memory")
+        for t in (k, v):
+            for s in (k_scale, v_scale):
+                at = s.data_ptr() - t.data_ptr()
+                _need(not _meets(dims, at - HEAD_DIM, at + s.nbytes),
+                      "Q8Cache: codes and scales must not share memory")
         self.k, self.v, self.k_scale, self.v_scale, self.block = k, v, k_scale, v_scale, block
         self.batch, self.kv_heads, self.capacity, self.device = B, H, S, k.device
         self._c = _lib.NkQ8Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),

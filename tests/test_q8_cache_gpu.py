@@ -579,3 +579,43 @@ def test_attention_all_idle_in_a_long_cache(B):
     q = rand(2 * B, 16 * 128, seed=B)
     assert (run_attention(q, cache, [-1 - b for b in range(B)], 16) == 0).all()
     assert nk.device_error() == 0
+
+
+def test_cache_refuses_arrays_that_overlap_at_an_offset():
+    f8 = torch.float8_e4m3fn
+    c = ops.Q8Cache.empty(2, 2, 64, DEV)
+    n = c.k.numel()
+    flat = torch.zeros(2 * n, dtype=torch.uint8, device=DEV)
+
+    def codes(start):
+        return flat[start:start + n].view(2, 2, 64, 128).view(f8)
+
+    ops.Q8Cache(codes(0), codes(n), c.k_scale, c.v_scale, 64)
+    for start in (16, 128, 64 * 128, n - 16):
+        for k, v in ((0, start), (start, 0)):
+            with pytest.raises(ValueError, match="k and v must not share"):
+                ops.Q8Cache(codes(k), codes(v), c.k_scale, c.v_scale, 64)
+    # rows of 256 bytes: the values between the keys' rows, or half over them
+    pair = torch.zeros(2, 2, 64, 2, 128, dtype=torch.uint8, device=DEV)
+    k = pair[..., 0, :].view(f8)
+    for at, fine in ((128, True), (64, False), (192, False), (256, False)):
+        v = pair.view(-1)[at:].as_strided((2, 2, 64, 128), k.stride()).view(f8) if at <= 128 else \
+            torch.zeros(pair.numel() + 512, dtype=torch.uint8, device=DEV)
+        if at > 128:
+            v, k2 = (v[o:].as_strided((2, 2, 64, 128), k.stride()).view(f8) for o in (at, 0))
+        else:
+            k2 = k
+        if fine:
+            ops.Q8Cache(k2, v, c.k_scale, c.v_scale, 64)
+        else:
+            with pytest.raises(ValueError, match="k and v must not share"):
+                ops.Q8Cache(k2, v, c.k_scale, c.v_scale, 64)
+    s = torch.zeros(8, device=DEV)
+    ops.Q8Cache(c.k, c.v, s[:4].view(2, 2, 1), s[4:].view(2, 2, 1), 64)
+    with pytest.raises(ValueError, match="k_scale and v_scale must not share"):
+        ops.Q8Cache(c.k, c.v, s[:4].view(2, 2, 1), s[3:7].view(2, 2, 1), 64)
+    inside = flat[n - 16:n].view(torch.float32).view(2, 2, 1)
+    with pytest.raises(ValueError, match="codes and scales must not share"):
+        ops.Q8Cache(codes(0), codes(n), inside, c.v_scale, 64)
+    with pytest.raises(ValueError, match="codes and scales must not share"):
+        ops.Q8Cache(codes(0), codes(n), c.k_scale, inside, 64)

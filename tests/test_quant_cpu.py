@@ -212,3 +212,30 @@ def test_withhold_w4_request_rejects_a_bad_cta():
     L = _lib.load()
     assert L.nk_test_withhold_w4(-2) == _lib.NK_ERR_ARG
     assert L.nk_test_withhold_w4(-1) == 0
+
+
+def test_rows_of_two_arrays_meet_or_not():
+    """The search that Q8Cache refuses overlapping arrays by, against all sums."""
+    g = torch.Generator().manual_seed(7)
+
+    def some(lo, hi):
+        return int(torch.randint(lo, hi, (1,), generator=g))
+
+    met = 0
+    for _ in range(3000):
+        dims, extent = [], 4
+        for _ in range(some(0, 4)):  # each stride past what is below it, as a cache's are
+            stride, count = extent + some(0, 9), some(2, 5)
+            dims.insert(0, (stride, count))
+            extent = stride * count
+        both = [(st, 2 * n - 1) for st, n in dims]
+        for d in (dims, both):
+            sums = [0]
+            for st, n in d:
+                sums = [x + i * st for x in sums for i in range(n)]
+            lo = some(-20, 2 * extent + 20)
+            hi = lo + some(1, 30)
+            want = any(lo < x < hi for x in sums)
+            assert ops._meets(d, lo, hi) == want, (d, lo, hi)
+            met += want
+    assert 1000 < met < 5000
