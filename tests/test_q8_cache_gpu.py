@@ -619,3 +619,33 @@ def test_cache_refuses_arrays_that_overlap_at_an_offset():
         ops.Q8Cache(codes(0), codes(n), inside, c.v_scale, 64)
     with pytest.raises(ValueError, match="codes and scales must not share"):
         ops.Q8Cache(codes(0), codes(n), c.k_scale, inside, 64)
+
+
+@pytest.mark.parametrize("B,T,heads,kv,block", [(16, 16, 32, 8, 32), (64, 4, 24, 8, 16), (200, 1, 28, 4, 64)])
+@pytest.mark.parametrize("std", (1.0, 1e-3))
+def test_append_rounds_as_64_bits_do(B, T, heads, kv, block, std):
+    """Queries and key codes equal those of a norm in 64 bits, every one of them.
+
+    The kernel's normalised value is x times 1 / rms as a pair of floats, with the product's own error
+    added: within some 2^-46 of the exact one before it is rounded to fp32, as the 64-bit value is on its
+    way to bf16. The two fp32 values differ where the exact one lies within 2^-46 of the middle between two
+    of them, 2^-21 of all (some 1 of the 10^6 here), and bf16 shows that for one in 2^16 of those. A norm
+    in fp32 (errors of 2^-24 and more) moves one value in 10^4 or so across a bf16 border."""
+    S = 128
+    cache = ops.Q8Cache.empty(B, kv, S, DEV, block=block)
+    qkv = rand(B * T, (heads + 2 * kv) * 128, std=std, seed=B)
+    cos, sin = tables(S)
+    qn, kn = (torch.rand(128, generator=gen(i), device=DEV).add(0.5).to(torch.bfloat16) for i in (60, 61))
+    pos = [(7 * b) % (S // block) * block for b in range(B)]  # the first slots of a block
+    q_out = append(cache, qkv, heads, pos, cos, sin, qn, kn)
+    rows = qkv.view(B, T, heads + 2 * kv, 128).double()
+    at = torch.tensor(pos, device=DEV)[:, None] + torch.arange(T, device=DEV)
+    c, s = cos[at].double()[:, :, None], sin[at].double()[:, :, None]
+    assert torch.equal(q_out.view(B, T, heads, 128).double(), rows_ref(rows[:, :, :heads], qn, c, s))
+    keys = rows_ref(rows[:, :, heads:heads + kv], kn, c, s)
+    amax = keys.abs().amax(dim=(1, 3))  # of the new tokens, all of one block
+    scale = torch.exp2(torch.ceil(torch.log2(amax / 448.0)).clamp(min=-64))
+    b = torch.arange(B, device=DEV)
+    assert torch.equal(cache.k_scale[b, :, torch.tensor(pos, device=DEV) // block].double(), scale)
+    got = cache.k[b[:, None], :, at].double()  # [B, T, kv, 128]
+    assert torch.equal(got, e4m3(keys / scale[:, None, :, None]))
