@@ -649,3 +649,36 @@ def test_append_rounds_as_64_bits_do(B, T, heads, kv, block, std):
     assert torch.equal(cache.k_scale[b, :, torch.tensor(pos, device=DEV) // block].double(), scale)
     got = cache.k[b[:, None], :, at].double()  # [B, T, kv, 128]
     assert torch.equal(got, e4m3(keys / scale[:, None, :, None]))
+
+
+def test_each_refusal_is_its_own():
+    """Every bad argument beside three good ones, and the message that names it."""
+    c = filled_cache(2, 2, 64, 16)
+    k, v, ks, vs = c.k, c.v, c.k_scale, c.v_scale
+    ops.Q8Cache(k, v, ks, vs, 16)
+
+    def refused(match, **bad):
+        with pytest.raises(ValueError, match=match):
+            ops.Q8Cache(**(dict(k=k, v=v, k_scale=ks, v_scale=vs, block=16) | bad))
+
+    refused("float8_e4m3fn", k=k.view(torch.uint8))
+    refused("float8_e4m3fn", v=v.view(torch.uint8))
+    refused("float8_e4m3fn", k=k[..., :64])
+    refused("float8_e4m3fn", k=k[0])
+    refused("float8_e4m3fn", v=torch.zeros_like(v.view(torch.uint8), device="cpu").view(v.dtype))
+    refused("same shape", v=v[:1])
+    refused("same shape", v=torch.zeros(2, 64, 2, 128, dtype=torch.uint8, device=DEV).transpose(1, 2).view(v.dtype))
+    refused("block must be", block=24)
+    refused("scales must be", block=32)
+    refused("scales must be", k_scale=ks[:, :, :1])
+    refused("scales must be", v_scale=vs.double())
+    refused("scales must be", v_scale=vs.cpu())
+    refused("scales must be", k_scale=ks.transpose(0, 1))
+    refused("layout", k=k[:, :1].expand(2, 2, 64, 128), v=v[:, :1].expand(2, 2, 64, 128))
+    refused("layout", k=k[:1].expand(2, 2, 64, 128), v=v[:1].expand(2, 2, 64, 128))
+    wide = torch.zeros(2, 2, 2, 64, 136, dtype=torch.uint8, device=DEV).view(k.dtype)
+    refused("layout", k=wide[0, ..., :128], v=wide[1, ..., :128])  # strides of 136
+    wide = torch.zeros(2, 2, 2, 64, 144, dtype=torch.uint8, device=DEV).view(k.dtype)
+    ops.Q8Cache(wide[0, ..., :128], wide[1, ..., :128], ks, vs, 16)
+    refused("layout", k=wide[0, ..., 8:136], v=wide[1, ..., 8:136])  # addresses of 8
+    refused("batch 1", k=k[:0], v=v[:0], k_scale=ks[:0], v_scale=vs[:0])
