@@ -682,3 +682,24 @@ def test_each_refusal_is_its_own():
     ops.Q8Cache(wide[0, ..., :128], wide[1, ..., :128], ks, vs, 16)
     refused("layout", k=wide[0, ..., 8:136], v=wide[1, ..., 8:136])  # addresses of 8
     refused("batch 1", k=k[:0], v=v[:0], k_scale=ks[:0], v_scale=vs[:0])
+
+
+def test_largest_batch():
+    B, S, T = ops.Q8_MAX_BATCH, 90, 2
+    cache = filled_cache(B, 1, S, 32, seed=20)
+    pos = [(37 * b) % (S - T + 1) if b % 5 else -1 for b in range(B)]
+    check_append(cache, rand(B * T, 4 * 128, seed=21), 2, pos, T)
+    out = check_attention(rand(B * T, 2 * 128, seed=22), cache, pos, 2)
+    assert (out.view(B, -1)[::5] == 0).all()
+    with pytest.raises(ValueError, match="batch 1"):
+        ops.Q8Cache.empty(B + 1, 1, 16, DEV)
+    assert nk.device_error() == 0
+
+
+def test_largest_head_counts_and_drafts():
+    heads, kv, T = 4096, 256, 16
+    cache = filled_cache(1, kv, 40, 16, seed=23)
+    check_append(cache, rand(T, (heads + 2 * kv) * 128, seed=24), heads, [13], T)
+    check_attention(rand(T, heads * 128, seed=25), cache, [13], heads)
+    with pytest.raises(ValueError):
+        ops.attention_q8_workspace(filled_cache(1, 257, 16, 16), 257 * 16)

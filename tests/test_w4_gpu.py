@@ -208,3 +208,15 @@ def test_withhold_request_is_validated():
     nk.mm_w4(x, W, out=y)
     check(y, x, w)
     assert nk.device_error() == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(70000, 130, 200), (1 << 20, 3, 16)])
+def test_many_tokens(M, N, K):
+    W, w = make(N, K, 32, True, torch.bfloat16)
+    x = synthetic.activation(M, K, seed=1, device=DEV)
+    y = torch.full((M, N), float("nan"), dtype=torch.bfloat16, device=DEV)
+    nk.mm_w4(x, W, out=y)
+    check(y, x, w)
+    if M == 1 << 20:
+        with pytest.raises(ValueError):
+            nk.mm_w4(torch.cat((x, x[:1])), W, out=torch.cat((y, y[:1])))
