@@ -2,7 +2,7 @@
  * nk_quant.h — the quantised decode step of libnkgemm.so (sm_100a): linears with 4-bit weights,
  * and a KV cache held in 8 bits with the append that fills it and the attention that reads it.
  * They stand beside nk_gemm_bf16 (nk_gemm.h), nk_qk_norm_rope_cache_bf16 and
- * nk_attention_decode_bf16 (nk_decode.h), move a quarter and half of their bytes, and share
+ * nk_attention_decode_bf16 (nk_decode.h), read a quarter and half of their bytes, and share
  * their conventions: device pointers, a cudaStream_t, 0 or NK_ERR_* returned before anything is
  * launched, no allocation, no host synchronisation, capture-safe, programmatic dependent launch.
  * The reference engine is bf16 throughout and has no counterpart of these.
@@ -53,8 +53,9 @@ NK_API size_t nk_w4_scale_bytes(int N, int K, int group);
 NK_API size_t nk_w4_zero_bytes(int N, int K, int group);
 
 /* x: [M, K] bf16, row stride ldx >= K (elements); y: [M, N] bf16, row stride ldy >= N; both 2-byte
- * aligned (x 16-byte aligned with ldx % 8 == 0 is read by TMA); y not in x's memory. Any M from 1 to 2^20. No
- * workspace. The weights must have been written before the launch that precedes this one on the
+ * aligned (x 16-byte aligned with ldx % 8 == 0 is read by TMA, others by a slower copy); y not in x's
+ * memory. Any M from 1 to 2^20; the weights are read and widened once per 64 rows of x, so past some
+ * 128 rows (64 with groups of 32) nk_gemm_bf16 is the faster linear. No workspace. The weights must have been written before the launch that precedes this one on the
  * stream (they are read ahead of it); weights made at load time always are. */
 NK_API int nk_gemm_w4(const void* x, int64_t ldx, const nk_w4_weight* w, void* y, int64_t ldy,
                       int M, nk_stream_t stream);
@@ -122,9 +123,14 @@ NK_API int nk_qk_norm_rope_cache_q8(const void* qkv, int64_t ld_qkv, const void*
 NK_API size_t nk_attention_q8_ws_bytes(int tokens, int q_heads, int kv_heads);
 
 /* Grouped attention of the new tokens over the cache: query row (b, t, h) sees slots
- * 0 .. position + t of kv head h / (q_heads / kv_heads); fp32 scores, softmax and sums, rounded
- * once to bf16; rows of idle sequences are zero. q, out: [batch * tokens, q_heads * 128] bf16,
- * 8-byte aligned. q_heads / kv_heads between 1 and 16; ws 16-byte aligned. */
+ * 0 .. position + t of kv head h / (q_heads / kv_heads); rows of idle sequences are zero. Scores,
+ * softmax and sums in fp32, the result rounded once to bf16. The matrix instructions take f16 on the way:
+ *   probabilities rounded to 11 bits down to 2^-22 of the row's largest, to 2^-33 of it below that
+ *   (blocks whose value scale is less than 2^-64 of the largest one lose more);
+ *   a query row as it is, save that elements below 2^-29 of its largest (of 2^-88, where that is
+ *   more) keep fewer bits, and may keep none below 2^-37 of it.
+ * q, out: [batch * tokens, q_heads * 128] bf16, 8-byte aligned. q_heads / kv_heads between 1 and 16;
+ * ws 16-byte aligned. */
 NK_API int nk_attention_decode_q8(const void* q, const nk_q8_cache* cache,
                                   const int64_t* position, int per_sequence, void* out, int tokens,
                                   int q_heads, float scale, void* ws, size_t ws_bytes,

@@ -22,12 +22,14 @@ __device__ __forceinline__ int64_t q8_position(const int64_t* position, int per_
 // row (lane l owns elements 4l .. 4l + 3; its RoPE partner is lane l ^ 16).
 //
 // A CTA of eight warps takes either query rows (one or four a warp, their loads in flight
-// together), or one (sequence, kv head, touched block): it holds the block's new rows in registers (at most 16 tokens, two a warp), finds their
-// largest magnitudes, fixes the block's two scales, rounds earlier tokens' codes anew where a
-// scale rose, and stores. Each block belongs to one CTA, so nothing is shared between CTAs. A
-// few hundred KB move at most; the launch and two dependent round trips to memory bound it (2.7 us
-// at one token, 0.75 where every sequence is idle; 7.5 us at 16 sequences of 16 tokens and 64
-// heads, 1.3 TB/s).
+// together), or one (sequence, kv head, touched block): it holds the block's new rows in registers
+// (at most 16 tokens, two a warp), finds their largest magnitudes, fixes the block's two scales, rounds
+// earlier tokens' codes anew where a scale rose, and stores. Each block belongs to one CTA, so nothing
+// is shared between CTAs. The launch and two dependent round trips to memory bound it at one token (2.8
+// us, 0.75 where every sequence is idle; 16 sequences 3.2), issue slots at 16 sequences of 16 tokens and
+// 64 heads (7.5 us for 10 MB, 1.3 TB/s). Where a scale rises, a warp takes one earlier row after the
+// other, each a load, a conversion and a store: 6.5 us where a full block of 64 is rounded anew, 9.5
+// for one of 128, against 3.2 measured the same way where none rises.
 // ---------------------------------------------------------------------------------------
 struct Q8AppendArgs {
     const __nv_bfloat16* qkv; int64_t ld;
@@ -293,8 +295,8 @@ __global__ void __launch_bounds__(32 * kQ8Warps) q8_append_kernel(const Q8Append
 // 30 at five of 3000 with 32 query rows: one CTA walks through all rows of the pair.)
 //
 // Measured, 8 kv heads (us, all launches; in brackets the cache's bytes at 6456 GB/s): two
-// sequences of 128k slots 85.5 [83.2], 6.3 TB/s; 16 ragged ones of up to 8192 slots 31.5 [22.0]; one
-// of 1024 slots (a cluster per pair) 5.0 [0.3]; five of up to 2999, four tokens x 64 heads, 18.8
+// sequences of 128k slots 85.3 [83.2], 6.3 TB/s; 16 ragged ones of up to 8192 slots 31.4 [22.0]; one
+// of 1024 slots (a cluster per pair) 5.1 [0.3]; five of up to 2999, four tokens x 64 heads, 18.3
 // [2.8]. Long caches stream at the copy rate; the fixed part (first bytes, join, two launches) is
 // some 4 to 6 us; many query rows are bound by the conversions and the matrix instructions (issue
 // slots 45% busy at 12 warps an SM).
@@ -1001,8 +1003,10 @@ static bool q8_block_ok(int block) {
     return block == 16 || block == 32 || block == 64 || block == 128;
 }
 // Query rows of one CTA: one or two column tiles of eight. More rows take several CTAs, which read
-// the cache again (from L2): measured against four tiles a CTA, 19.8 us against 22.4 (five
-// sequences of 3000 slots, 32 rows), 185 against 177 (16 of 8192, 64 rows).
+// the cache again (from L2) and widen it again. Four tiles a CTA leave two CTAs an SM: measured (us, two
+// tiles / four) 22.7 / 33.1 at 32 rows (five sequences of 2999 slots), 199 / 179 at 64 rows and 392 /
+// 342 at 128 (16 of 8192), 25.1 / 20.3 at 128 (two of 2048). So two serve drafts of up to 32 rows a kv
+// head, and lose 10 to 19% at 64 and more, where what costs is the widening either way.
 static int q8_rows(int rows) { return rows <= 8 ? 8 : 16; }
 
 // The short-cache form: one launch of a cluster per pair.
@@ -1190,10 +1194,10 @@ extern "C" int nk_attention_decode_q8(const void* q, const nk_q8_cache* c,
     cudaStream_t s = (cudaStream_t)stream;
     // The short-cache form with the largest cluster that leaves every CTA resident (384 of them, in
     // clusters, at three CTAs an SM), if a CTA then has at most 512 slots to walk. Measured (us, one
-    // launch / two): 8 pairs 5.0 / 6.0 at 1024 slots, 8.6 / 8.9 at 4096, 10.7 / 10.7 at 6000; 64 pairs
-    // (clusters of 4) 7.9 / 10.0 at 1024, 12.1 / 12.9 at 2048, 18.8 / 18.2 at 4096; 128 pairs (of 2)
-    // 7.7 / 9.8 at 512, 11.9 / 12.8 at 1024, 18.7 / 18.3 at 2048; past one wave, 64 pairs in
-    // clusters of 8, 15.2 / 12.9 at 2048.
+    // launch / two): 8 pairs 5.1 / 6.1 at 1024 slots, 9.3 / 9.7 at 4096, 11.6 / 11.5 at 6000; 64 pairs
+    // (clusters of 4) 8.5 / 11.3 at 1024, 12.3 / 13.8 at 2048, 18.8 / 18.2 at 4096; 128 pairs (of 2)
+    // 8.4 / 11.2 at 512, 12.1 / 13.5 at 1024, 18.8 / 18.4 at 2048; past one wave, 64 pairs in
+    // clusters of 8, 16.0 / 13.8 at 2048.
     const int64_t pairs = (int64_t)a.batch * a.hkv * a.row_blocks;
     for (int lg = 3; lg > 0 && !a.lg_cluster; --lg)
         if (pairs << lg <= 384) a.lg_cluster = lg;

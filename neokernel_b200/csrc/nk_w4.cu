@@ -15,15 +15,18 @@
 // MMA's A operand there (128 rows = 128 lanes), the tokens its B operand in shared memory.
 //
 // Measured in CUDA graphs (us; in brackets the weight bytes' time at 6456 GB/s, the copy rate):
-//   N 24576, K 4096   M=1 16.1 [8.0], M=64 24.8 [8.3]     group 128
-//   N 6144, K 4096    M=16 7.8 [2.1]                      group 64
+//   N 24576, K 4096   M=1 16.1 [8.0], M=64 24.9 [8.3]     group 128
+//   N 6144, K 4096    M=16 8.0 [2.1]                      group 64
 //   N 4096, K 12288   M=8 11.6 [4.7]                      group 32 with zero points
 //   N 1024, K 2048    M=1 3.4 [0.2]: the launch and one pass through the pipeline
 // Per step of 128 x 128 the eight MMAs take some 256 cycles (each reads 4 KB of A from tensor
 // memory at 128 bytes a cycle), and a step of a CTA 450 to 500, with its barriers. So what bounds
 // the wide shapes is the time per step on the SMs that hold two CTAs while others hold one (192
 // row tiles on 148 SMs), the narrow ones the fixed parts (some 3 us: launch, first bytes, the
-// cluster's sum). On mma.sync, with the weights widened in registers, the same cases took 14.2
+// cluster's sum). Against this library's bf16 linear (30.8 us at N 24576, K 4096, M=1) it is ahead up
+// to 64 tokens (24.3 against 36.6 at group 128, 31.5 at 64) but for groups of 32 (45.4 at 64 tokens), and
+// behind from some 128 on, as the weights are widened again for every 64: at M=128, 37.5, 48.9 and 70.8
+// us (groups 128, 64, 32) against 41.8; at 256, 70, 91 and 130 against 67.5. On mma.sync, with the weights widened in registers, the same cases took 14.2
 // (M=1), 75 (M=64), 12 and 19 us.
 //
 // A CTA takes 128 weight rows and a range of K steps (128 wide). Its warps:

@@ -368,7 +368,9 @@ def attention_decode_q8(q, cache: Q8Cache, position, out, ws, heads: int,
     """``attention_decode`` of T = 1..16 new tokens per sequence over a ``Q8Cache`` that already
     holds them: row b * T + t of q, out [batch * T, heads * 128] attends over slots
     [0, position[b] + t]. ``position`` as in ``qk_norm_rope_cache_q8``; rows of idle sequences
-    come out zero. ``heads`` is 1 to 16 times the cache's kv_heads."""
+    come out zero. ``heads`` is 1 to 16 times the cache's kv_heads. fp32 throughout but for the
+    probabilities and the queries as the matrix instructions take them (f16; include/nk_quant.h says
+    what that keeps)."""
     name = "attention_decode_q8"
     T = _q8_tokens(q, cache, heads * HEAD_DIM, "attention_decode_q8: q")
     if _q8_tokens(out, cache, heads * HEAD_DIM, "attention_decode_q8: out") != T \

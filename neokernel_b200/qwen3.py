@@ -190,7 +190,8 @@ class Qwen3W4Weights:
 
 def quantize_linears(w: Qwen3Weights, group: int = 128, zeros: bool = False) -> Qwen3W4Weights:
     """The model with its layer linears rounded to 4 bits (scales in bf16 per ``group`` of K, and
-    with ``zeros`` a zero point each). Decode it with ``linear=w4.linear, fused=True``."""
+    with ``zeros`` a zero point each). Decode it with ``linear=w4.linear, fused=True``, on one GPU:
+    the tensor-parallel hooks (tp.make_hooks) refuse 4-bit weights."""
     return Qwen3W4Weights(w, group, zeros)
 
 

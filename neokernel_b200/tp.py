@@ -118,7 +118,8 @@ def make_hooks(w: TPWeights, group=None, linear_f32=None, linear=None, collectiv
     to ``FUSED_MAX_M``, else all_reduce. ``fused_head`` (CUDA states only)
     takes each rank's (max, lowest index) from the lm_head launch (``neokernel_b200.mm_argmax``)
     instead of storing the logits and reducing them; ``state.logits`` is then left untouched.
-    Buffers are allocated here, once per state, so the hooks are capture-safe.
+    Buffers are allocated here, once per state, so the hooks are capture-safe. Weights are bf16: a
+    ``W4Weight`` has no unrounded partial to sum and is refused (``ValueError``).
     """
     if collective not in ("auto", "fused", "peer", "nccl"):
         raise ValueError(f"collective must be auto, fused, peer or nccl, not {collective!r}")

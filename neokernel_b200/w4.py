@@ -158,8 +158,9 @@ def mm_w4(a: torch.Tensor, w: W4Weight, *, out: torch.Tensor,
 
     a: bf16 CUDA [M, K] with unit column stride; out: bf16 CUDA [M, N] with unit column stride, in
     memory that ``a`` does not share.
-    Any M; made for decode batches and drafts of up to 64 tokens (larger ones read the weights once
-    per 64 tokens).
+    Any M; made for decode batches and drafts of up to 64 tokens. Larger ones read and widen the
+    weights once per 64 tokens: from some 128 tokens on (64 with groups of 32) ``mm`` with the bf16
+    weight is faster, and a model that is not short of memory keeps that for them.
     """
     if not isinstance(w, W4Weight):
         raise ValueError(f"mm_w4: w must be a W4Weight, got {type(w).__name__}")
@@ -201,7 +202,9 @@ def mm_w4(a: torch.Tensor, w: W4Weight, *, out: torch.Tensor,
 
 def linear(a: torch.Tensor, b, *, out: torch.Tensor) -> torch.Tensor:
     """``out = a @ b`` for a ``W4Weight`` (``mm_w4``) or a bf16 ``W.t()`` (``mm``): the ``linear``
-    of a decode step whose layers are in 4 bits and whose lm_head is not."""
+    of a decode step whose layers are in 4 bits and whose lm_head is not. (The tensor-parallel
+    hooks sum unrounded partials of o_proj and down, which ``mm_w4`` does not give: they take bf16
+    weights.)"""
     if isinstance(b, W4Weight):
         return mm_w4(a, b, out=out)
     return mm(a, b, out=out)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import neokernel_b200 as nk
-from neokernel_b200 import qwen3, w4
+from neokernel_b200 import qwen3, tp, w4
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -100,3 +100,25 @@ def test_refusals():
     st = qwen3.DecodeState(w, 1, 16, cache="e4m3")
     with pytest.raises(ValueError):
         qwen3.decode_step(st, w, nk.mm, fused=False)
+
+
+def test_tensor_parallel_hooks_refuse_4_bit_weights():
+    w = tp.TPWeights(DIMS, 3, 0, 1)
+    _, q = models()
+    st = qwen3.DecodeState(w, 2, 16)
+    row_linear, _ = tp.make_hooks(w)(st)
+    st.attn.zero_()
+    row_linear(st.attn, w.layers[0].o, st.branch)
+    with pytest.raises(ValueError, match="torch.Tensor"):
+        row_linear(st.attn, q.layers[0].o, st.branch)
+
+
+def test_tensor_parallel_hooks_over_an_8_bit_cache():
+    """One rank: its shard is the whole model, so the tokens are those of the single-GPU step."""
+    w, _ = models()
+    t = tp.TPWeights(DIMS, 3, 0, 1)
+    prompt = torch.randint(0, DIMS.vocab, (2, 6), device=DEV)
+    ref = qwen3.GraphDecoder(w, 2, 64, nk.mm, fused=True, cache="e4m3").greedy(prompt, 30)
+    got = qwen3.GraphDecoder(t, 2, 64, nk.mm, make_hooks=tp.make_hooks(t), fused=True,
+                             cache="e4m3").greedy(prompt, 30)
+    assert torch.equal(ref, got)
